@@ -274,6 +274,135 @@ int ssmap_ego_maps(ssmap_engine *eng, const double *agent_pose, const int32_t *g
 int ssmap_path_append(ssmap_engine *eng, int32_t e, const int32_t *cells, int32_t n, void *stream);
 int ssmap_path_paint(ssmap_engine *eng, void *stream);
 
+/* ---- Head operators: what a model's last layer computes and how likely the given labels are under it.
+ *
+ * They belong to no engine: the caller passes device pointers, shapes and strides (in elements), a
+ * stream of the current device and, where ssmap_*_workspace() asks for one, a workspace that is used by
+ * this call alone until its work on the stream is done.  Nothing is allocated, nothing waits, nothing is
+ * kept between calls, so a call may be captured into a graph and replayed.  No counterpart in the
+ * reference, whose networks end in library calls (infer.py:95-118, 301-327 hold what follows them).
+ *
+ * Two layouts.  SSMAP_ROWS: the classes lie last, [batch][rows][classes], as a language model leaves its
+ * logits.  SSMAP_PLANES: one plane per class, [batch][classes][rows], as a segmentation head leaves them
+ * and as ssmap_frames.logits wants them.  "position" below is one (batch, row) pair. */
+typedef enum ssmap_dtype { SSMAP_F32 = 0, SSMAP_BF16 = 1, SSMAP_F16 = 2 } ssmap_dtype;
+typedef enum ssmap_layout { SSMAP_ROWS = 0, SSMAP_PLANES = 1 } ssmap_layout;
+typedef enum ssmap_activation {
+    SSMAP_ACT_NONE = 0,
+    SSMAP_ACT_RELU = 1,       /* max(z, 0); its slope at 0 is 0 */
+    SSMAP_ACT_GELU = 2,       /* z (1 + erf(z / sqrt 2)) / 2 */
+    SSMAP_ACT_GELU_TANH = 3,  /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+    SSMAP_ACT_SILU = 4        /* z / (1 + exp(-z)) */
+} ssmap_activation;
+
+#define SSMAP_MAX_TOP 32      /* most alternatives per position */
+
+/* Log probabilities of given ids.  With z = logits / temperature, per position:
+ *   row_max = max logit, log_sum = log sum_j exp((logit_j - row_max) / temperature),
+ *   log_prob = z_id - log sum_j exp z_j,   entropy = -sum_j p_j log p_j (nats),
+ *   top_ids / top_log_prob: the `top` largest logits, ties to the lowest class.
+ * An id equal to ignore_id has log_prob 0; any other id outside [0, classes) has log_prob NaN.
+ * A logit of -inf is a masked class: probability 0, never an alternative (id -1, log probability -inf
+ * where fewer than `top` classes are left).  A position whose classes are all masked has row_max, log_sum
+ * and log_prob -inf and entropy 0.  A position that holds a NaN or +inf has no distribution: log_prob
+ * (unless ignored), entropy, log_sum and top_log_prob are NaN, its top_ids -1. */
+typedef struct ssmap_log_probs_args {
+    int32_t dtype, layout;             /* of the logits */
+    int64_t batch, rows, classes;      /* batch and rows may be 0; classes >= 1 */
+    const void *logits;                /* class stride 1 in rows, row stride 1 in planes */
+    int64_t batch_stride;              /* of the logits */
+    int64_t inner_stride;              /* rows: of a row; planes: of a plane */
+    const void *ids;                   /* [batch][rows], int32 or int64 */
+    int64_t ids_batch_stride, ids_row_stride;
+    int64_t ignore_id;
+    int32_t ids_64;                    /* the ids are int64 */
+    int32_t top;                       /* 0 ... min(SSMAP_MAX_TOP, classes) */
+    float temperature;                 /* 1e-30 ... 1e30 */
+    int32_t pad;
+    float *log_prob, *entropy, *row_max, *log_sum;   /* [batch][rows], dense */
+    int32_t *top_ids;                  /* rows: [batch][rows][top]; planes: [batch][top][rows]; dense */
+    float *top_log_prob;
+    void *workspace;
+    int64_t workspace_bytes;
+} ssmap_log_probs_args;
+int64_t ssmap_log_probs_workspace(const ssmap_log_probs_args *args);   /* bytes; looks at the sizes only; -1: bad sizes */
+int ssmap_log_probs(const ssmap_log_probs_args *args, void *stream);
+
+/* The gradient with respect to the logits of sum (g_log_prob log_prob + g_entropy entropy +
+ * g_top top_log_prob):
+ *   d / d logit_j = ( g_l ([j = id] - p_j) + sum_k g_top_k ([j = top_id_k] - p_j)
+ *                     - g_e p_j (log p_j + entropy) ) / temperature.
+ * row_max, log_sum, entropy and top_ids are ssmap_log_probs' answers for the same logits.  Ignored ids
+ * and alternatives of id -1 give nothing.  A position whose classes are all masked has the gradient 0;
+ * one without a distribution, or with an id outside [0, classes) and a g_log_prob given, NaN.  A
+ * gradient that is NULL counts as 0. */
+typedef struct ssmap_log_probs_grad_args {
+    int32_t dtype, layout;
+    int64_t batch, rows, classes;
+    const void *logits;
+    int64_t batch_stride, inner_stride;
+    const void *ids;
+    int64_t ids_batch_stride, ids_row_stride;
+    int64_t ignore_id;
+    int32_t ids_64, top;
+    float temperature;
+    int32_t pad;
+    const float *row_max, *log_sum, *entropy;        /* [batch][rows], dense */
+    const int32_t *top_ids;                          /* as ssmap_log_probs wrote them; may be NULL when top is 0 */
+    const float *g_log_prob, *g_entropy, *g_top;     /* dense, or NULL */
+    void *grad;                                      /* out, dense in the logits' layout and type */
+} ssmap_log_probs_grad_args;
+int ssmap_log_probs_grad(const ssmap_log_probs_grad_args *args, void *stream);
+
+/* y = act(x w^T + bias) + residual.  x [batch][rows][inner], w [outer][inner]; y, residual and pre are
+ * [batch][rows][outer] in rows, [batch][outer][rows] in planes.  Products of 16-bit values are summed in
+ * 32 bits, in an order that the sizes alone decide; the sum is rounded once, to out_dtype.  `pre`, if
+ * given, receives x w^T + bias (rounded to dtype), which ssmap_linear_grad needs where there is an
+ * activation. */
+typedef struct ssmap_linear_args {
+    int32_t dtype;                     /* of x, w and pre */
+    int32_t out_dtype;                 /* of y and residual: dtype or SSMAP_F32 */
+    int32_t activation, layout;
+    int64_t batch, rows, inner, outer; /* each may be 0 */
+    const void *x;                     /* element stride 1 */
+    int64_t x_batch_stride, x_row_stride;
+    const void *w;                     /* element stride 1 */
+    int64_t w_row_stride;
+    const void *bias;                  /* [outer] dense, or NULL */
+    int32_t bias_dtype;                /* dtype or SSMAP_F32 */
+    int32_t pad;
+    const void *residual;              /* or NULL; last stride 1 */
+    int64_t res_batch_stride, res_inner_stride;   /* inner: of a row (rows) or a plane (planes) */
+    void *y, *pre;                     /* dense; pre or NULL */
+    void *workspace;
+    int64_t workspace_bytes;
+} ssmap_linear_args;
+int64_t ssmap_linear_workspace(const ssmap_linear_args *args);
+int ssmap_linear(const ssmap_linear_args *args, void *stream);
+
+/* The gradients of ssmap_linear from g = dL/dy.  With dz = g act'(pre):
+ *   g_x = dz w,   g_w = dz^T x,   g_bias = sum of dz over the positions   (g itself is the residual's).
+ * dz is rounded to dtype before the two products (their operands are the matrix instructions' types) and
+ * summed unrounded for g_bias.  Outputs that are NULL are left out. */
+typedef struct ssmap_linear_grad_args {
+    int32_t dtype;                     /* of x, w, pre and the outputs */
+    int32_t grad_dtype;                /* of g: dtype or SSMAP_F32 */
+    int32_t activation, layout;
+    int64_t batch, rows, inner, outer;
+    const void *g;                     /* last stride 1 */
+    int64_t g_batch_stride, g_inner_stride;
+    const void *pre;                   /* dense like y; NULL without an activation */
+    const void *x;
+    int64_t x_batch_stride, x_row_stride;
+    const void *w;
+    int64_t w_row_stride;
+    void *g_x, *g_w, *g_bias;          /* dense [batch][rows][inner], [outer][inner], [outer] */
+    void *workspace;
+    int64_t workspace_bytes;
+} ssmap_linear_grad_args;
+int64_t ssmap_linear_grad_workspace(const ssmap_linear_grad_args *args);
+int ssmap_linear_grad(const ssmap_linear_grad_args *args, void *stream);
+
 const char *ssmap_last_error(void);
 const char *ssmap_version(void);
 

@@ -19,7 +19,9 @@ ENV_INDEX_ERROR = 1
 EXPORTS = ("ssmap_create", "ssmap_destroy", "ssmap_set_schema", "ssmap_set_palette",
            "ssmap_set_params", "ssmap_bind_env", "ssmap_step", "ssmap_step_noalloc", "ssmap_stage1",
            "ssmap_read_results", "ssmap_gt_goal_query", "ssmap_update_list", "ssmap_profile_begin", "ssmap_profile_read",
-           "ssmap_set_egomap", "ssmap_ego_maps", "ssmap_set_nb_model", "ssmap_path_append", "ssmap_path_paint", "ssmap_last_error", "ssmap_version")
+           "ssmap_set_egomap", "ssmap_ego_maps", "ssmap_set_nb_model", "ssmap_path_append", "ssmap_path_paint",
+           "ssmap_log_probs_workspace", "ssmap_log_probs", "ssmap_log_probs_grad", "ssmap_linear_workspace", "ssmap_linear",
+           "ssmap_linear_grad_workspace", "ssmap_linear_grad", "ssmap_last_error", "ssmap_version")
 
 
 class Config(C.Structure):
@@ -70,6 +72,36 @@ class EgomapConfig(C.Structure):
                 ("active_goal_color", C.c_uint8 * 3), ("arrow_color", C.c_uint8 * 3), ("pad", C.c_uint8 * 2)]
 
 
+def _fields(text):
+    """ctypes fields from "name:kind" words; kinds: i int32, q int64, f float, p pointer."""
+    kinds = {"i": C.c_int32, "q": C.c_int64, "f": C.c_float, "p": C.c_void_p}
+    return [(n, kinds[k]) for n, k in (w.split(":") for w in text.split())]
+
+
+class LogProbsArgs(C.Structure):
+    _fields_ = _fields("dtype:i layout:i batch:q rows:q classes:q logits:p batch_stride:q inner_stride:q ids:p "
+                       "ids_batch_stride:q ids_row_stride:q ignore_id:q ids_64:i top:i temperature:f pad:i log_prob:p "
+                       "entropy:p row_max:p log_sum:p top_ids:p top_log_prob:p workspace:p workspace_bytes:q")
+
+
+class LogProbsGradArgs(C.Structure):
+    _fields_ = _fields("dtype:i layout:i batch:q rows:q classes:q logits:p batch_stride:q inner_stride:q ids:p "
+                       "ids_batch_stride:q ids_row_stride:q ignore_id:q ids_64:i top:i temperature:f pad:i row_max:p "
+                       "log_sum:p entropy:p top_ids:p g_log_prob:p g_entropy:p g_top:p grad:p")
+
+
+class LinearArgs(C.Structure):
+    _fields_ = _fields("dtype:i out_dtype:i activation:i layout:i batch:q rows:q inner:q outer:q x:p x_batch_stride:q "
+                       "x_row_stride:q w:p w_row_stride:q bias:p bias_dtype:i pad:i residual:p res_batch_stride:q "
+                       "res_inner_stride:q y:p pre:p workspace:p workspace_bytes:q")
+
+
+class LinearGradArgs(C.Structure):
+    _fields_ = _fields("dtype:i grad_dtype:i activation:i layout:i batch:q rows:q inner:q outer:q g:p g_batch_stride:q "
+                       "g_inner_stride:q pre:p x:p x_batch_stride:q x_row_stride:q w:p w_row_stride:q g_x:p g_w:p g_bias:p "
+                       "workspace:p workspace_bytes:q")
+
+
 def load():
     """Returns the loaded library; raises if it was not built (python semantic-search_amd/build.py)."""
     global _lib
@@ -103,11 +135,16 @@ def load():
     lib.ssmap_set_nb_model.argtypes = [vp, i32, i32, vp, vp, vp, vp, vp]
     lib.ssmap_path_append.argtypes = [vp, i32, vp, i32, vp]
     lib.ssmap_path_paint.argtypes = [vp, vp]
+    for name, args in (("log_probs", LogProbsArgs), ("log_probs_grad", LogProbsGradArgs), ("linear", LinearArgs),
+                       ("linear_grad", LinearGradArgs)):
+        getattr(lib, "ssmap_" + name).argtypes = [C.POINTER(args), vp]
+        if name != "log_probs_grad":
+            getattr(lib, f"ssmap_{name}_workspace").argtypes = [C.POINTER(args)]
     lib.ssmap_last_error.restype = C.c_char_p
     lib.ssmap_version.restype = C.c_char_p
     for name in EXPORTS:
         if name not in ("ssmap_destroy", "ssmap_last_error", "ssmap_version"):
-            getattr(lib, name).restype = C.c_int
+            getattr(lib, name).restype = C.c_int64 if name.endswith("_workspace") else C.c_int
     _lib = lib
     return lib
 

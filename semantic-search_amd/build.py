@@ -24,6 +24,8 @@ SOURCES = [
     ("label.hip", ["-ffp-contract=off"]),
     ("ego.hip", ["-ffp-contract=off"]),
     ("fuse.hip", []),
+    ("scores.hip", []),
+    ("linear.hip", []),
     ("engine.cpp", ["-ffp-contract=off"]),
 ]
 COMMON = ["-x", "hip", "-O3", "--offload-arch=gfx950", "-std=c++17", "-fPIC",
@@ -40,6 +42,7 @@ def _newer(target, deps):
 def build(force: bool = False, verbose: bool = True) -> str:
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     headers = [os.path.join(CSRC, "ssmap_internal.h"), os.path.join(CSRC, "rows.h"),
+               os.path.join(CSRC, "heads.h"),
                os.path.join(ROOT, "include", "ssmap.h")]
     os.makedirs(LIB_DIR, exist_ok=True)
     os.makedirs(OBJ_DIR, exist_ok=True)

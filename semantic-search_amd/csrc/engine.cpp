@@ -11,6 +11,7 @@
 #include <type_traits>
 #include <vector>
 
+#include "heads.h"
 #include "ssmap_internal.h"
 
 using namespace ssmap;
@@ -211,6 +212,15 @@ static void predict_box(const ssmap_config &c, const ssmap_env_maps &mp, PoseBlo
     b.box[2] = std::max(cell(lo_x, mp.lower[0]) - 2, -mp.map_w);
     b.box[3] = std::min(cell(hi_x, mp.lower[0]) + 2, mp.map_w - 1);
     if (b.box[0] > b.box[1] || b.box[2] > b.box[3]) { b.box[0] = b.box[2] = 0; b.box[1] = b.box[3] = -1; }
+}
+
+int ssmap::head_error(int code, const char *text) noexcept {
+    try {
+        g_error = text;
+    } catch (...) {   // no memory for the text: the code alone goes back
+        g_error.clear();
+    }
+    return code;
 }
 
 extern "C" {

@@ -14,7 +14,7 @@ from typing import Dict, Optional, Sequence
 import numpy as np
 import torch
 
-from . import _capi
+from . import _capi, heads
 
 AVG_RULES = ("avg_prob", "w_avg_prob", "w2_avg_prob")
 PROB_RULES = AVG_RULES + ("log_odds",)
@@ -139,6 +139,7 @@ class MapEngine:
         self.maps: list[Optional[Dict[str, torch.Tensor]]] = [None] * self.n_envs
         self.map_bounds: list[Optional[np.ndarray]] = [None] * self.n_envs
         self._keep = None
+        self._head = None
 
     # ------------------------------------------------------------------ egocentric maps
     def set_egomap(self, egomap_small_side_m: float = 3.0, egomap_large_side_m: float = 10.0,
@@ -326,14 +327,38 @@ class MapEngine:
         self.map_bounds[e] = b
         return m
 
+    # ---- the segmentation network's last layer
+    def set_head(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None):
+        """The network's class head: weight [n_classes, D] (float32, bfloat16 or float16, on the engine's
+        device), bias [n_classes] in its type or float32.  Kept by reference, for `head_logits` and
+        `step(features=...)`."""
+        if weight.dim() != 2 or weight.shape[0] != self.n_classes or weight.device != self.device:
+            raise ValueError(f"weight: expected [{self.n_classes}, D] on {self.device}, got {tuple(weight.shape)} on {weight.device}")
+        if bias is not None and tuple(bias.shape) != (self.n_classes,):
+            raise ValueError(f"bias: expected ({self.n_classes},), got {tuple(bias.shape)}")
+        self._head = (weight, bias)
+
+    def head_logits(self, features: torch.Tensor) -> torch.Tensor:
+        """float32 class planes [E, C, H, W] = features [E, H, W, D] times the head, for `step` and `stage1`."""
+        if self._head is None:
+            raise RuntimeError("set_head was not called")
+        weight, bias = self._head
+        shape = (self.n_envs, self.img_h, self.img_w, weight.shape[1])
+        if tuple(features.shape) != shape:
+            raise ValueError(f"features: expected {shape}, got {tuple(features.shape)}")
+        return heads.linear(features, weight, bias, planes=True, out_dtype=torch.float32)
+
     # ---- one batch of frames
     def step(self, depth: torch.Tensor, agent_pose, camera_pose, goal_sem_ids, *,
              logits: Optional[torch.Tensor] = None, probs: Optional[torch.Tensor] = None,
              temperature: float = 1.0, semantic: Optional[torch.Tensor] = None,
              semantic_unc: Optional[torch.Tensor] = None,
              semantic_max_prob: Optional[torch.Tensor] = None,
-             semantic_gt: Optional[torch.Tensor] = None, static_scratch: bool = False, skip=None):
-        """Enqueues stages 1-5 for all envs on the current stream.  `skip` (host bools [E]) names envs
+             semantic_gt: Optional[torch.Tensor] = None, static_scratch: bool = False, skip=None,
+             features: Optional[torch.Tensor] = None):
+        """Enqueues stages 1-5 for all envs on the current stream.  Instead of `logits` the `features`
+        [E, H, W, D] of the network's last layer may be given, in the type of the head that `set_head`
+        took: the head's product then comes first (see `head_logits`).  `skip` (host bools [E]) names envs
         without a frame in this batch: their maps and state stay untouched, their results read
         found False, status 0, 0 updates.  With `static_scratch` the
         allocation-free entry point runs the step (per-step scratch in the library's file-scope
@@ -350,6 +375,10 @@ class MapEngine:
                                  f"got {t.dtype} {tuple(t.shape)} on {t.device}")
             return t.data_ptr()
 
+        if features is not None:
+            if logits is not None or probs is not None:
+                raise ValueError("features: logits or probs are given as well")
+            logits = self.head_logits(features)
         fr = _capi.Frames()
         fr.depth = dev(depth, torch.float32, (E, H, W), "depth")
         fr.logits = dev(logits, torch.float32, (E, self.n_classes, H, W), "logits")
