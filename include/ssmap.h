@@ -308,7 +308,7 @@ typedef enum ssmap_activation {
  * (unless ignored), entropy, log_sum and top_log_prob are NaN, its top_ids -1. */
 typedef struct ssmap_log_probs_args {
     int32_t dtype, layout;             /* of the logits */
-    int64_t batch, rows, classes;      /* batch and rows may be 0; classes >= 1 */
+    int64_t batch, rows, classes;      /* batch, rows >= 0, batch * rows < 2^31; 1 <= classes <= 2^30 */
     const void *logits;                /* class stride 1 in rows, row stride 1 in planes */
     int64_t batch_stride;              /* of the logits */
     int64_t inner_stride;              /* rows: of a row; planes: of a plane */

@@ -16,6 +16,7 @@ using namespace ssmap;
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int64_t kMostBlocks = 1 << 22;   // a grid holds fewer than 2^32 threads; kernels loop over what is beyond
 constexpr float kLn2 = 0.693147180559945309f, kLog2e = 1.44269504088896341f;
 constexpr float kTiny = -200.0f;   // 2^-200 is 0 in float: exponents are clamped to it where 0 * -inf would be NaN
 
@@ -79,80 +80,6 @@ __device__ __forceinline__ float top_value(const Shape &s, Best v, const Said &w
     return w.bad ? __builtin_nanf("") : !(v.v > -INFINITY) ? -INFINITY : (v.v - w.row_max) * s.inv_t - kLn2 * w.log2_s;
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-    for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
-    return v;
-}
-__device__ __forceinline__ float wave_sum(float v) {
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-    return v;
-}
-__device__ __forceinline__ Best wave_best(Best v) {
-    for (int d = 1; d < 64; d <<= 1) {
-        const Best w{__shfl_xor(v.v, d), __shfl_xor(v.i, d)};
-        if (better(w, v)) v = w;
-    }
-    return v;
-}
-
-// One block per position, the classes read three times and once more for each alternative.
-template <int DT>
-__global__ __launch_bounds__(kThreads) void k_scores(Shape s, const elem_t<DT> *logits, const void *ids, Out o) {
-    __shared__ float part[2][kThreads / 64];
-    __shared__ Best best[kThreads / 64];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-    for (int64_t pos = blockIdx.x; pos < s.batch * s.rows; pos += gridDim.x) {
-        const int64_t b = pos / s.rows, r = pos % s.rows;
-        const elem_t<DT> *row = logits + b * s.batch_stride + r * s.row_stride;
-        float m = -INFINITY;
-        for (int64_t j = tid; j < s.classes; j += kThreads) m = fmaxf(m, Elem<DT>::get(row[j * s.class_stride]));
-        m = wave_max(m);
-        __syncthreads();
-        if (!lane) part[0][wave] = m;
-        __syncthreads();
-        for (int w = 0; w < kThreads / 64; ++w) m = fmaxf(m, part[0][w]);
-        __syncthreads();
-        const float ms = m == -INFINITY ? 0.0f : m;
-        float sum = 0.0f, wsum = 0.0f;
-        for (int64_t j = tid; j < s.classes; j += kThreads) {
-            const float t = (Elem<DT>::get(row[j * s.class_stride]) - ms) * s.scale, e = __builtin_amdgcn_exp2f(t);
-            sum += e;
-            wsum += e * fmaxf(t, kTiny);
-        }
-        sum = wave_sum(sum);
-        wsum = wave_sum(wsum);
-        if (!lane) part[0][wave] = sum, part[1][wave] = wsum;
-        __syncthreads();
-        sum = wsum = 0.0f;
-        for (int w = 0; w < kThreads / 64; ++w) sum += part[0][w], wsum += part[1][w];
-        const int64_t id = load_id(s, ids, b, r);
-        const float xid = id >= 0 && id < s.classes ? Elem<DT>::get(row[id * s.class_stride]) : 0.0f;
-        const Said said = say(s, m, sum, wsum, id, xid);
-        if (!tid) put(o, pos, said);
-        Best last{INFINITY, -1};
-        for (int k = 0; k < s.top; ++k) {
-            Best mine{-INFINITY, kNoId};
-            for (int64_t j = tid; j < s.classes; j += kThreads) {
-                const Best v{Elem<DT>::get(row[j * s.class_stride]), (int32_t)j};
-                if (better(last, v) && better(v, mine)) mine = v;
-            }
-            mine = wave_best(mine);
-            __syncthreads();
-            if (!lane) best[wave] = mine;
-            __syncthreads();
-            for (int w = 0; w < kThreads / 64; ++w)
-                if (better(best[w], mine)) mine = best[w];
-            if (!tid) {
-                const int64_t at = top_at(s, b, r, k);
-                o.top_ids[at] = top_id(mine, said);
-                o.top_log_prob[at] = top_value(s, mine, said);
-            }
-            last = mine;
-        }
-        __syncthreads();
-    }
-}
-
 // What is loaded at once: N neighbours at any element alignment.
 template <int DT, int N>
 struct Pack {
@@ -166,6 +93,308 @@ __device__ __forceinline__ Pack<DT, N> load_pack(const elem_t<DT> *p) {
 }
 template <int DT, int N>
 __device__ __forceinline__ void store_pack(elem_t<DT> *p, const Pack<DT, N> &r) { __builtin_memcpy(p, &r, sizeof r); }
+
+// Running sums of a set of classes relative to its own maximum.
+struct Sums {
+    float m, sum, wsum;
+};
+__device__ __forceinline__ Sums join(const Shape &s, const Sums &a, const Sums &b) {
+    const float m = fmaxf(a.m, b.m), ms = m == -INFINITY ? 0.0f : m;
+    const float da = fmaxf((a.m - ms) * s.scale, kTiny), db = fmaxf((b.m - ms) * s.scale, kTiny);
+    const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
+    return {m, fa * a.sum + fb * b.sum, fa * (a.wsum + a.sum * da) + fb * (b.wsum + b.sum * db)};
+}
+template <int LANES>
+__device__ __forceinline__ Sums lanes_join(const Shape &s, Sums v) {
+    float m = v.m;
+#pragma unroll
+    for (int d = 1; d < LANES; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+    const float ms = m == -INFINITY ? 0.0f : m, dv = fmaxf((v.m - ms) * s.scale, kTiny), f = __builtin_amdgcn_exp2f(dv);
+    v = {m, f * v.sum, f * (v.wsum + v.sum * dv)};
+#pragma unroll
+    for (int d = 1; d < LANES; d <<= 1) v.sum += __shfl_xor(v.sum, d), v.wsum += __shfl_xor(v.wsum, d);
+    return v;
+}
+
+// Short rows: LPR lanes hold a row in registers (NP packs a lane), so the maximum is known before the sums
+// and each alternative is found by one more look at the registers.
+template <int DT, int LPR, int NP>
+__global__ __launch_bounds__(kThreads) void k_scores_short(Shape s, const elem_t<DT> *logits, const void *ids, Out o) {
+    constexpr int VEC = 16 / sizeof(elem_t<DT>), UNITS = kThreads / LPR;
+    const int sub = threadIdx.x % LPR;
+    const int64_t n = s.batch * s.rows;
+    // every lane stays in the loop as long as its block has a row: the exchanges below need all of a wave
+    for (int64_t first = blockIdx.x * (int64_t)UNITS; first < n; first += (int64_t)gridDim.x * UNITS) {
+        const int64_t mine = first + threadIdx.x / LPR, pos = mine < n ? mine : n - 1;
+        const int64_t b = pos / s.rows, r = pos % s.rows;
+        const elem_t<DT> *row = logits + b * s.batch_stride + r * s.row_stride;
+        float x[NP][VEC];
+#pragma unroll
+        for (int u = 0; u < NP; ++u) {
+            const int64_t j = (u * LPR + sub) * VEC;
+            if (j + VEC <= s.classes) {
+                const Pack<DT, VEC> v = load_pack<DT, VEC>(row + j);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) x[u][e] = Elem<DT>::get(v.v[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) x[u][e] = j + e < s.classes ? Elem<DT>::get(row[j + e]) : -INFINITY;
+            }
+        }
+        const int64_t id = load_id(s, ids, b, r);
+        const float xid = id >= 0 && id < s.classes ? Elem<DT>::get(row[id]) : 0.0f;
+        float m = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < NP; ++u)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) m = fmaxf(m, x[u][e]);
+#pragma unroll
+        for (int d = 1; d < LPR; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+        const float ms = m == -INFINITY ? 0.0f : m;
+        float sum = 0.0f, wsum = 0.0f;
+#pragma unroll
+        for (int u = 0; u < NP; ++u)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float t = (x[u][e] - ms) * s.scale, p = __builtin_amdgcn_exp2f(t);
+                sum += p;
+                wsum += p * fmaxf(t, kTiny);
+            }
+#pragma unroll
+        for (int d = 1; d < LPR; d <<= 1) sum += __shfl_xor(sum, d), wsum += __shfl_xor(wsum, d);
+        const Said said = say(s, m, sum, wsum, id, xid);
+        const bool writes = sub == 0 && mine < n;
+        if (writes) put(o, pos, said);
+        Best last{INFINITY, -1};
+        for (int k = 0; k < s.top; ++k) {
+            Best best{-INFINITY, kNoId};
+#pragma unroll
+            for (int u = 0; u < NP; ++u)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {   // the lane's classes ascend: an equal value never replaces
+                    const Best v{x[u][e], (int32_t)((u * LPR + sub) * VEC + e)};
+                    if (better(last, v) && v.v > best.v) best = v;
+                }
+#pragma unroll
+            for (int d = 1; d < LPR; d <<= 1) {
+                const Best w{__shfl_xor(best.v, d), __shfl_xor(best.i, d)};
+                if (better(w, best)) best = w;
+            }
+            if (writes) {
+                o.top_ids[pos * s.top + k] = top_id(best, said);
+                o.top_log_prob[pos * s.top + k] = top_value(s, best, said);
+            }
+            last = best;
+        }
+    }
+}
+
+constexpr int kLongPacks = 4;               // packs a thread of a long row has in flight
+constexpr int kCandidates = kThreads * 8 + SSMAP_MAX_TOP;   // one gathering step's most, and the best so far
+
+// A block's alternatives: candidates in any order (their keys differ, so the order of the atomics does not
+// matter), ranked by counting.
+struct Candidates {
+    Best list[kCandidates];
+    Best kept[SSMAP_MAX_TOP];
+    int count;
+};
+__device__ __forceinline__ void offer(Candidates &c, const Best &v) { c.list[atomicAdd(&c.count, 1)] = v; }
+// The best `top` of the list into kept[], in order; all threads call it.
+__device__ __forceinline__ void rank_candidates(Candidates &c, int top) {
+    __syncthreads();
+    const int n = c.count;
+    if (threadIdx.x < top) c.kept[threadIdx.x] = Best{-INFINITY, kNoId};
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const Best v = c.list[i];
+        int rank = 0;
+        for (int q = 0; q < n; ++q) rank += better(c.list[q], v);
+        if (rank < top) c.kept[rank] = v;
+    }
+    __syncthreads();
+}
+
+struct Part {       // what a segment of a split row says, followed by `top` alternatives
+    Sums sums;
+    float pad;
+};
+
+// Long rows: a block takes one segment of a row, in one pass over memory.  Each thread keeps running sums of
+// its packs (rescaled once a pack) and where its largest logit first stood.  At the end the `top` threads
+// with the best maxima hold every alternative: any other thread's logits are beaten by those `top` maxima
+// (values first; among equal ones the thread whose pack comes first wins, and its pack lies in front of the
+// other's).  Only their packs are read again, from the caches, and only what is at least the last of the
+// maxima becomes a candidate.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void k_scores_long(Shape s, const elem_t<DT> *logits, const void *ids, Out o, int splits, int64_t segment, char *parts, int64_t part_bytes) {
+    constexpr int VEC = 16 / sizeof(elem_t<DT>), U = kLongPacks, STEP = kThreads * VEC;
+    __shared__ Sums joint[kThreads / 64];
+    __shared__ Best firsts[kThreads];
+    __shared__ int chosen[SSMAP_MAX_TOP];
+    __shared__ Candidates cand;
+    const int tid = threadIdx.x;
+    for (int64_t unit = blockIdx.x; unit < s.batch * s.rows * splits; unit += gridDim.x) {
+        const int64_t pos = unit / splits, b = pos / s.rows, r = pos % s.rows;
+        const int64_t from = unit % splits * segment, to = from + segment < s.classes ? from + segment : s.classes;
+        const elem_t<DT> *row = logits + b * s.batch_stride + r * s.row_stride;
+        const auto fetch = [&](int64_t j, float (&x)[VEC]) {
+            if (j + VEC <= to) {
+                const Pack<DT, VEC> v = load_pack<DT, VEC>(row + j);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) x[e] = Elem<DT>::get(v.v[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) x[e] = j + e < to ? Elem<DT>::get(row[j + e]) : -INFINITY;
+            }
+        };
+        Sums v{-INFINITY, 0.0f, 0.0f};
+        Best first{-INFINITY, (int32_t)(from + tid * VEC)};
+        for (int64_t j0 = from + tid * VEC; j0 < to; j0 += U * STEP) {
+            float x[U][VEC];
+#pragma unroll
+            for (int u = 0; u < U; ++u) fetch(j0 + u * STEP, x[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float pm = x[u][0];
+#pragma unroll
+                for (int e = 1; e < VEC; ++e) pm = fmaxf(pm, x[u][e]);
+                if (pm > first.v) first = Best{pm, (int32_t)(j0 + u * STEP)};
+                const float m = fmaxf(v.m, pm), ms = m == -INFINITY ? 0.0f : m;
+                const float d = fmaxf((v.m - ms) * s.scale, kTiny), f = __builtin_amdgcn_exp2f(d);
+                v.wsum = f * (v.wsum + v.sum * d);
+                v.sum *= f;
+                v.m = m;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float t = (x[u][e] - ms) * s.scale, p = __builtin_amdgcn_exp2f(t);
+                    v.sum += p;
+                    v.wsum += p * fmaxf(t, kTiny);
+                }
+            }
+        }
+        v = lanes_join<64>(s, v);
+        __syncthreads();
+        if (tid % 64 == 0) joint[tid / 64] = v;
+        firsts[tid] = first;
+        if (!tid) cand.count = 0;
+        __syncthreads();
+        v = joint[0];
+        for (int w = 1; w < kThreads / 64; ++w) v = join(s, v, joint[w]);
+        if (s.top) {
+            int rank = 0;
+            for (int q = 0; q < kThreads; ++q) rank += better(firsts[q], first);
+            if (rank < s.top) chosen[rank] = tid;
+            __syncthreads();
+            const Best least = firsts[chosen[s.top - 1]];
+            const int64_t packs = (to - from + STEP - 1) / STEP, items = packs * s.top;
+            for (int64_t i0 = 0; i0 < items; i0 += kThreads) {
+                const int have = cand.count;
+                __syncthreads();   // nobody offers before everybody has read the count
+                if (have > kCandidates - kThreads * VEC) {
+                    rank_candidates(cand, s.top);
+                    if (tid < s.top) cand.list[tid] = cand.kept[tid];
+                    if (!tid) cand.count = s.top;
+                    __syncthreads();
+                }
+                const int64_t i = i0 + tid;
+                if (i < items) {
+                    const int64_t j = from + (i / s.top * kThreads + chosen[i % s.top]) * VEC;
+                    float x[VEC];
+                    fetch(j, x);
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e)
+                        if (x[e] > -INFINITY && (x[e] > least.v || (x[e] == least.v && j + e < least.i + VEC))) offer(cand, Best{x[e], (int32_t)(j + e)});
+                }
+                __syncthreads();
+            }
+            rank_candidates(cand, s.top);
+        }
+        if (splits > 1) {
+            char *part = parts + unit * part_bytes;
+            if (!tid) reinterpret_cast<Part *>(part)->sums = v;
+            if (tid < s.top) reinterpret_cast<Best *>(part + sizeof(Part))[tid] = cand.kept[tid];
+        } else {
+            const int64_t id = load_id(s, ids, b, r);
+            const float xid = id >= 0 && id < s.classes ? Elem<DT>::get(row[id]) : 0.0f;
+            const Said said = say(s, v.m, v.sum, v.wsum, id, xid);
+            if (!tid) put(o, pos, said);
+            if (tid < s.top) {
+                o.top_ids[pos * s.top + tid] = top_id(cand.kept[tid], said);
+                o.top_log_prob[pos * s.top + tid] = top_value(s, cand.kept[tid], said);
+            }
+        }
+    }
+}
+
+// Joins the segments of a split row: one block per row, at most kThreads segments.  The `top` segments with
+// the best first alternatives hold all of the row's.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void k_scores_join(Shape s, const elem_t<DT> *logits, const void *ids, Out o, int splits, const char *parts, int64_t part_bytes) {
+    __shared__ Sums joint[kThreads / 64];
+    __shared__ Best firsts[kThreads], least;
+    __shared__ Candidates cand;
+    const int tid = threadIdx.x;
+    for (int64_t pos = blockIdx.x; pos < s.batch * s.rows; pos += gridDim.x) {
+        const int64_t b = pos / s.rows, r = pos % s.rows;
+        const char *part = parts + (pos * splits + (tid < splits ? tid : 0)) * part_bytes;
+        const Best *list = reinterpret_cast<const Best *>(part + sizeof(Part));
+        Sums v{-INFINITY, 0.0f, 0.0f};
+        Best first{-INFINITY, kNoId};
+        if (tid < splits) {
+            v = reinterpret_cast<const Part *>(part)->sums;
+            if (s.top) first = list[0];
+        }
+        v = lanes_join<64>(s, v);
+        __syncthreads();
+        if (tid % 64 == 0) joint[tid / 64] = v;
+        firsts[tid] = first;
+        if (!tid) cand.count = 0, least = Best{-INFINITY, kNoId};
+        __syncthreads();
+        v = joint[0];
+        for (int w = 1; w < kThreads / 64; ++w) v = join(s, v, joint[w]);
+        if (s.top) {
+            int rank = 0;
+            for (int q = 0; q < splits; ++q) rank += better(firsts[q], first);
+            if (tid < splits && rank == s.top - 1 && first.v > -INFINITY) least = first;
+            __syncthreads();
+            if (tid < splits && rank < s.top)
+                for (int k = 0; k < s.top; ++k) {
+                    const Best c = list[k];
+                    if (!(c.v > -INFINITY) || better(least, c)) break;
+                    offer(cand, c);
+                }
+            rank_candidates(cand, s.top);
+        }
+        const elem_t<DT> *row = logits + b * s.batch_stride + r * s.row_stride;
+        const int64_t id = load_id(s, ids, b, r);
+        const float xid = id >= 0 && id < s.classes ? Elem<DT>::get(row[id]) : 0.0f;
+        const Said said = say(s, v.m, v.sum, v.wsum, id, xid);
+        if (!tid) put(o, pos, said);
+        if (tid < s.top) {
+            o.top_ids[pos * s.top + tid] = top_id(cand.kept[tid], said);
+            o.top_log_prob[pos * s.top + tid] = top_value(s, cand.kept[tid], said);
+        }
+    }
+}
+
+// Segments of a long row: one where the rows alone fill the card (two blocks a CU), otherwise enough for
+// four, each at least one pack a thread.
+struct Split {
+    int splits;
+    int64_t segment, part_bytes;
+};
+inline Split split_rows(const Shape &s, int dtype) {
+    const int64_t n = s.batch * s.rows, step = kThreads * (16 / head_dtype_size(dtype));
+    Split w{1, s.classes, (int64_t)(sizeof(Part) + s.top * sizeof(Best))};
+    if (n == 0 || n >= 512 || s.classes <= step) return w;
+    int64_t most = (s.classes + step - 1) / step;
+    most = most < 1024 / n ? most : 1024 / n;
+    most = most < kThreads ? most : kThreads;
+    w.segment = ((s.classes + most - 1) / most + step - 1) / step * step;
+    w.splits = (int)((s.classes + w.segment - 1) / w.segment);
+    return w;
+}
 
 // Sorted alternatives in registers: K values with their classes, `j` later than every class in the list, so
 // an equal value goes behind.  slot q becomes the middle of (slot q-1, slot q, v).
@@ -277,40 +506,80 @@ struct Grads {
     const int32_t *top_ids;
 };
 
-// One block per position.
-template <int DT>
-__global__ __launch_bounds__(kThreads) void k_scores_grad(Shape s, const elem_t<DT> *logits, const void *ids, Grads g, elem_t<DT> *grad) {
-    for (int64_t pos = blockIdx.x; pos < s.batch * s.rows; pos += gridDim.x) {
-        const int64_t b = pos / s.rows, r = pos % s.rows;
+constexpr int kGradPacks = 4;   // packs of 16 bytes a lane has in flight
+
+// Rows: LPR lanes take kGradPacks packs each of one row, one pass.  d = p (A + B t) with t = log2 p, plus
+// g_l at the given class; alternatives, at most 32 places of a row, are computed again and stored over the
+// row afterwards by the lanes that wrote it.
+template <int DT, int LPR>
+__global__ __launch_bounds__(kThreads) void k_grad_rows(Shape s, const elem_t<DT> *logits, const void *ids, Grads g, elem_t<DT> *grad) {
+    constexpr int VEC = 16 / sizeof(elem_t<DT>), U = kGradPacks, UNITS = kThreads / LPR;
+    const int sub = threadIdx.x % LPR;
+    const int64_t chunks = (s.classes + LPR * VEC * U - 1) / (LPR * VEC * U), units = s.batch * s.rows * chunks;
+    for (int64_t unit = blockIdx.x * (int64_t)UNITS + threadIdx.x / LPR; unit < units; unit += (int64_t)gridDim.x * UNITS) {
+        const int64_t pos = unit / chunks, b = pos / s.rows, r = pos % s.rows;
+        const int64_t c0 = unit % chunks * (LPR * VEC * U), j0 = c0 + sub * VEC;
         const elem_t<DT> *row = logits + b * s.batch_stride + r * s.row_stride;
-        elem_t<DT> *out = s.layout == SSMAP_ROWS ? grad + pos * s.classes : grad + b * s.classes * s.rows + r;
-        const int64_t out_stride = s.layout == SSMAP_ROWS ? 1 : s.rows;
-        const int64_t id = load_id(s, ids, b, r);
-        const float m = g.row_max[pos], log2_s = g.log_sum[pos] * kLog2e;
-        const bool none = m == -INFINITY;
-        float g_l = g.g_log_prob && id != s.ignore_id ? g.g_log_prob[pos] : 0.0f;
-        const bool bad = g.log_sum[pos] != g.log_sum[pos] || (g.g_log_prob && id != s.ignore_id && (id < 0 || id >= s.classes));
-        const float g_e = g.g_entropy ? g.g_entropy[pos] : 0.0f, h = g.g_entropy ? g.entropy[pos] : 0.0f;
-        float all = g_l;
-        const int top = g.g_top ? s.top : 0;
-        for (int k = 0; k < top; ++k) {
-            const int64_t at = top_at(s, b, r, k);
-            all += g.top_ids[at] >= 0 ? g.g_top[at] : 0.0f;
-        }
-        for (int64_t j = threadIdx.x; j < s.classes; j += kThreads) {
-            float d = 0.0f;
-            if (!none) {
-                const float t = (Elem<DT>::get(row[j * s.class_stride]) - m) * s.scale - log2_s;
-                const float p = __builtin_amdgcn_exp2f(t);
-                d = -p * (all + g_e * (kLn2 * fmaxf(t, kTiny) + h));
-                if (j == id) d += g_l;
-                for (int k = 0; k < top; ++k) {
-                    const int64_t at = top_at(s, b, r, k);
-                    if (g.top_ids[at] == j) d += g.g_top[at];
-                }
+        elem_t<DT> *out = grad + pos * s.classes;
+        Pack<DT, VEC> in[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t j = j0 + u * (LPR * VEC);
+            if (j + VEC <= s.classes) {
+                in[u] = load_pack<DT, VEC>(row + j);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (j + e < s.classes) in[u].v[e] = row[j + e];
             }
-            if (bad) d = __builtin_nanf("");
-            out[j * out_stride] = Elem<DT>::put(d * s.inv_t);
+        }
+        const int64_t want = load_id(s, ids, b, r);
+        const float log_sum = g.log_sum[pos];
+        float m = g.row_max[pos], off = log_sum * kLog2e;
+        const bool none = m == -INFINITY, given = g.g_log_prob && want != s.ignore_id, inside = want >= 0 && want < s.classes;
+        const bool bad = log_sum != log_sum || (given && !inside);
+        const int top = g.g_top && !none ? s.top : 0;
+        float gl = given ? g.g_log_prob[pos] : 0.0f, all = gl;
+        for (int k = 0; k < top; ++k) all += g.top_ids[pos * s.top + k] >= 0 ? g.g_top[pos * s.top + k] : 0.0f;
+        const float ge = g.g_entropy ? g.g_entropy[pos] : 0.0f, h = g.g_entropy ? g.entropy[pos] : 0.0f;
+        float A = -(all + ge * h) * s.inv_t, B = -ge * kLn2 * s.inv_t;
+        gl *= s.inv_t;
+        int64_t id = given && inside ? want : -1;
+        if (none) {   // every t is -inf and every p 0
+            m = off = A = B = 0.0f;
+            id = -1;
+        }
+        if (bad) A = __builtin_nanf("");
+        const auto dense = [&](float x) {
+            const float t = (x - m) * s.scale - off;
+            return __builtin_amdgcn_exp2f(t) * (A + B * fmaxf(t, kTiny));
+        };
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t j = j0 + u * (LPR * VEC);
+            const int64_t at = id - j;   // the given class within this pack
+            Pack<DT, VEC> w;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) w.v[e] = Elem<DT>::put(dense(Elem<DT>::get(in[u].v[e])) + (at == e ? gl : 0.0f));
+            if (j + VEC <= s.classes) {
+                store_pack<DT, VEC>(out + j, w);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e)
+                    if (j + e < s.classes) out[j + e] = w.v[e];
+            }
+        }
+        if (top) {
+            bool waited = false;
+            for (int k = sub; k < top; k += LPR) {
+                const int64_t c = g.top_ids[pos * s.top + k];
+                if (c < c0 || c >= c0 + LPR * VEC * U) continue;
+                if (!waited) {   // the stores above come from other lanes of this wave
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    waited = true;
+                }
+                out[c] = Elem<DT>::put(dense(Elem<DT>::get(row[c])) + (c == id ? gl : 0.0f) + g.g_top[pos * s.top + k] * s.inv_t);
+            }
         }
     }
 }
@@ -400,8 +669,8 @@ int check(const Args *a, Shape &s) {
     if (!head_dtype_ok(a->dtype)) return head_error(SSMAP_ERR_INVALID_ARG, "dtype is none of SSMAP_F32, SSMAP_BF16, SSMAP_F16");
     if (a->layout != SSMAP_ROWS && a->layout != SSMAP_PLANES)
         return head_error(SSMAP_ERR_INVALID_ARG, "layout is neither SSMAP_ROWS nor SSMAP_PLANES");
-    if (!head_sizes_ok(a->batch, a->rows, a->classes) || a->classes < 1 || a->classes > INT32_MAX - 1)
-        return head_error(SSMAP_ERR_INVALID_ARG, "batch, rows >= 0, 1 <= classes < 2^31 - 1 and fewer than 2^40 logits are required");
+    if (!head_sizes_ok(a->batch, a->rows, a->classes) || a->classes < 1 || a->classes > (1 << 30))
+        return head_error(SSMAP_ERR_INVALID_ARG, "batch, rows >= 0, 1 <= classes <= 2^30 and fewer than 2^40 logits are required");
     if (a->batch * a->rows > INT32_MAX) return head_error(SSMAP_ERR_UNSUPPORTED, "more than 2^31 - 1 positions");
     if (a->top < 0 || a->top > SSMAP_MAX_TOP || a->top > a->classes)
         return head_error(SSMAP_ERR_INVALID_ARG, "top must be in [0, min(32, classes)]");
@@ -445,8 +714,20 @@ void launch_scores(const Shape &s, const ssmap_log_probs_args &a, hipStream_t st
         });
         return;
     }
+    constexpr int VEC = 16 / sizeof(elem_t<DT>), NP = 64 / (VEC * sizeof(float));   // 16 floats of a row a lane
     const int64_t n = s.batch * s.rows;
-    k_scores<DT><<<dim3((unsigned)(n < (1 << 20) ? n : (1 << 20))), kThreads, 0, st>>>(s, x, a.ids, o);
+    const auto brief = [&](auto lpr, auto np) {
+        const int64_t blocks = (n + kThreads / lpr.value - 1) / (kThreads / lpr.value);
+        k_scores_short<DT, lpr.value, np.value><<<(unsigned)(blocks < kMostBlocks ? blocks : kMostBlocks), kThreads, 0, st>>>(s, x, a.ids, o);
+    };
+    if (s.classes <= 16 * VEC) return brief(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
+    if (s.classes <= 16 * VEC * NP) return brief(std::integral_constant<int, 16>{}, std::integral_constant<int, NP>{});
+    if (s.classes <= 64 * VEC * NP) return brief(std::integral_constant<int, 64>{}, std::integral_constant<int, NP>{});
+    const Split w = split_rows(s, DT);
+    char *parts = static_cast<char *>(a.workspace);
+    const int64_t units = n * w.splits;
+    k_scores_long<DT><<<(unsigned)(units < kMostBlocks ? units : kMostBlocks), kThreads, 0, st>>>(s, x, a.ids, o, w.splits, w.segment, parts, w.part_bytes);
+    if (w.splits > 1) k_scores_join<DT><<<(unsigned)n, kThreads, 0, st>>>(s, x, a.ids, o, w.splits, parts, w.part_bytes);
 }
 
 template <int DT>
@@ -460,8 +741,16 @@ void launch_grad(const Shape &s, const ssmap_log_probs_grad_args &a, hipStream_t
         });
         return;
     }
-    const int64_t n = s.batch * s.rows;
-    k_scores_grad<DT><<<dim3((unsigned)(n < (1 << 20) ? n : (1 << 20))), kThreads, 0, st>>>(s, x, a.ids, g, out);
+    constexpr int VEC = 16 / sizeof(elem_t<DT>);
+    const auto go = [&](auto lpr) {
+        constexpr int LPR = lpr.value, UNITS = kThreads / LPR;
+        const int64_t chunks = (s.classes + LPR * VEC * kGradPacks - 1) / (LPR * VEC * kGradPacks), units = s.batch * s.rows * chunks;
+        const int64_t blocks = (units + UNITS - 1) / UNITS;
+        k_grad_rows<DT, LPR><<<(unsigned)(blocks < kMostBlocks ? blocks : kMostBlocks), kThreads, 0, st>>>(s, x, a.ids, g, out);
+    };
+    // a quarter of a wave where it holds the whole row
+    if (s.classes <= 16 * VEC * kGradPacks) go(std::integral_constant<int, 16>{});
+    else go(std::integral_constant<int, 64>{});
 }
 
 }  // namespace
@@ -471,7 +760,10 @@ extern "C" {
 int64_t ssmap_log_probs_workspace(const ssmap_log_probs_args *a) {
     Shape s{};
     if (!a) { head_error(SSMAP_ERR_INVALID_ARG, "null argument"); return -1; }
-    return check(a, s) == SSMAP_OK ? 0 : -1;
+    if (check(a, s) != SSMAP_OK) return -1;
+    if (s.layout == SSMAP_PLANES) return 0;
+    const Split w = split_rows(s, a->dtype);
+    return w.splits > 1 ? s.batch * s.rows * w.splits * w.part_bytes : 0;
 }
 
 int ssmap_log_probs(const ssmap_log_probs_args *a, void *stream) {
@@ -481,7 +773,8 @@ int ssmap_log_probs(const ssmap_log_probs_args *a, void *stream) {
     if (s.batch * s.rows == 0) return SSMAP_OK;
     if (!a->logits || !a->ids || !a->log_prob || !a->entropy || !a->row_max || !a->log_sum || (a->top && (!a->top_ids || !a->top_log_prob)))
         return head_error(SSMAP_ERR_INVALID_ARG, "null argument");
-    if (a->workspace_bytes < ssmap_log_probs_workspace(a)) return head_error(SSMAP_ERR_INVALID_ARG, "the workspace is smaller than ssmap_log_probs_workspace says");
+    const int64_t need = ssmap_log_probs_workspace(a);
+    if (a->workspace_bytes < need || (need && !a->workspace)) return head_error(SSMAP_ERR_INVALID_ARG, "the workspace is smaller than ssmap_log_probs_workspace says");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (a->dtype == SSMAP_F32) launch_scores<SSMAP_F32>(s, *a, st);
     else if (a->dtype == SSMAP_BF16) launch_scores<SSMAP_BF16>(s, *a, st);

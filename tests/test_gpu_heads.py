@@ -114,6 +114,30 @@ def test_many_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("n", [1, 520])
+def test_crowded_alternatives(n, dtype):
+    """Rows whose large logits stand a fixed distance apart, so that a few threads of a block read all of
+    them and many logits pass for candidates; ascending, descending and equal ones beside them."""
+    V, top = 40000, 32
+    g = gen(n)
+    rows = torch.zeros((7, V))
+    for i, (stride, width) in enumerate([(2048, 8 * 31), (1024, 4 * 31), (2048, 8)]):
+        at = torch.arange(V) % stride < width
+        rows[i, at] = 5 + torch.randn(int(at.sum()), generator=g)
+    rows[3] = torch.arange(V) / 1000.0
+    rows[4] = -torch.arange(V) / 1000.0
+    rows[5] = 1.0
+    rows[6, torch.randint(0, V, (3000,), generator=g)] = 7.0
+    rows = rows.to(dtype)
+    x = torch.zeros((max(n, 7), V), dtype=dtype, device="cuda")
+    x[-7:] = rows.cuda()
+    ids = torch.arange(x.shape[0]) % 9
+    got = ssa.log_probs(x, ids.cuda(), top=top)
+    want = plain_scores(rows, ids[-7:], 1.0, top)
+    check_scores(ssa.LogProbs(*[t[-7:] for t in got]), want, V)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
 @pytest.mark.parametrize("E,V,hw,top", [(1, 1, (1, 1), 1), (2, 3, (1, 5), 3), (3, 8, (7, 9), 2), (2, 40, (16, 33), 3), (1, 150, (13, 21), 5),
                                         (2, 155, (5, 64), 32), (1, 300, (3, 11), 9), (1, 21, (64, 65), 0)])
 def test_planes(E, V, hw, top, dtype):
