@@ -37,6 +37,17 @@ struct Best {
 constexpr int32_t kNoId = 0x7FFFFFFF;
 __device__ __forceinline__ bool better(const Best &a, const Best &b) { return a.v > b.v || (a.v == b.v && a.i < b.i); }
 
+// The same order as one number: larger is better.  0 is no class.  -0 becomes 0: equal logits, equal values.
+using Key = unsigned long long;
+__device__ __forceinline__ Key key_of(float v, int32_t i) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);
+    return (Key)(b ^ (b >> 31 ? 0xFFFFFFFFu : 0x80000000u)) << 32 | (uint32_t)~i;
+}
+__device__ __forceinline__ Best best_of(Key k) {
+    const uint32_t b = (uint32_t)(k >> 32);
+    return k ? Best{__builtin_bit_cast(float, b ^ (b >> 31 ? 0x80000000u : 0xFFFFFFFFu)), (int32_t)~(uint32_t)k} : Best{-INFINITY, kNoId};
+}
+
 __device__ __forceinline__ int64_t load_id(const Shape &s, const void *ids, int64_t b, int64_t r) {
     const int64_t at = b * s.ids_batch_stride + r * s.ids_row_stride;
     return s.ids_64 ? static_cast<const int64_t *>(ids)[at] : (int64_t) static_cast<const int32_t *>(ids)[at];
@@ -104,16 +115,37 @@ __device__ __forceinline__ Sums join(const Shape &s, const Sums &a, const Sums &
     const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
     return {m, fa * a.sum + fb * b.sum, fa * (a.wsum + a.sum * da) + fb * (b.wsum + b.sum * db)};
 }
+// All lanes of a group of 16 (a DPP row) or of a wave get the result; the exchanges are symmetric, so every
+// lane computes the same bits.
+template <int N>
+__device__ __forceinline__ float ror(float v) {   // rotated by N lanes within 16
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + N, 0xf, 0xf, false));
+}
+template <int N>
+__device__ __forceinline__ int32_t ror(int32_t v) { return __builtin_amdgcn_update_dpp(0, v, 0x120 + N, 0xf, 0xf, false); }
+template <int LANES>
+__device__ __forceinline__ float lanes_max(float v) {
+    v = fmaxf(v, ror<8>(v)); v = fmaxf(v, ror<4>(v)); v = fmaxf(v, ror<2>(v)); v = fmaxf(v, ror<1>(v));
+    if constexpr (LANES == 64) v = fmaxf(v, __shfl_xor(v, 16)), v = fmaxf(v, __shfl_xor(v, 32));
+    return v;
+}
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+    v += ror<8>(v); v += ror<4>(v); v += ror<2>(v); v += ror<1>(v);
+    if constexpr (LANES == 64) v += __shfl_xor(v, 16), v += __shfl_xor(v, 32);
+    return v;
+}
+template <int LANES>
+__device__ __forceinline__ int32_t lanes_min(int32_t v) {
+    v = min(v, ror<8>(v)); v = min(v, ror<4>(v)); v = min(v, ror<2>(v)); v = min(v, ror<1>(v));
+    if constexpr (LANES == 64) v = min(v, __shfl_xor(v, 16)), v = min(v, __shfl_xor(v, 32));
+    return v;
+}
 template <int LANES>
 __device__ __forceinline__ Sums lanes_join(const Shape &s, Sums v) {
-    float m = v.m;
-#pragma unroll
-    for (int d = 1; d < LANES; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+    const float m = lanes_max<LANES>(v.m);
     const float ms = m == -INFINITY ? 0.0f : m, dv = fmaxf((v.m - ms) * s.scale, kTiny), f = __builtin_amdgcn_exp2f(dv);
-    v = {m, f * v.sum, f * (v.wsum + v.sum * dv)};
-#pragma unroll
-    for (int d = 1; d < LANES; d <<= 1) v.sum += __shfl_xor(v.sum, d), v.wsum += __shfl_xor(v.wsum, d);
-    return v;
+    return {m, lanes_sum<LANES>(f * v.sum), lanes_sum<LANES>(f * (v.wsum + v.sum * dv))};
 }
 
 // Short rows: LPR lanes hold a row in registers (NP packs a lane), so the maximum is known before the sums
@@ -148,8 +180,7 @@ __global__ __launch_bounds__(kThreads) void k_scores_short(Shape s, const elem_t
         for (int u = 0; u < NP; ++u)
 #pragma unroll
             for (int e = 0; e < VEC; ++e) m = fmaxf(m, x[u][e]);
-#pragma unroll
-        for (int d = 1; d < LPR; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+        m = lanes_max<LPR>(m);
         const float ms = m == -INFINITY ? 0.0f : m;
         float sum = 0.0f, wsum = 0.0f;
 #pragma unroll
@@ -160,8 +191,8 @@ __global__ __launch_bounds__(kThreads) void k_scores_short(Shape s, const elem_t
                 sum += p;
                 wsum += p * fmaxf(t, kTiny);
             }
-#pragma unroll
-        for (int d = 1; d < LPR; d <<= 1) sum += __shfl_xor(sum, d), wsum += __shfl_xor(wsum, d);
+        sum = lanes_sum<LPR>(sum);
+        wsum = lanes_sum<LPR>(wsum);
         const Said said = say(s, m, sum, wsum, id, xid);
         const bool writes = sub == 0 && mine < n;
         if (writes) put(o, pos, said);
@@ -175,11 +206,8 @@ __global__ __launch_bounds__(kThreads) void k_scores_short(Shape s, const elem_t
                     const Best v{x[u][e], (int32_t)((u * LPR + sub) * VEC + e)};
                     if (better(last, v) && v.v > best.v) best = v;
                 }
-#pragma unroll
-            for (int d = 1; d < LPR; d <<= 1) {
-                const Best w{__shfl_xor(best.v, d), __shfl_xor(best.i, d)};
-                if (better(w, best)) best = w;
-            }
+            const float bv = lanes_max<LPR>(best.v);
+            best = Best{bv, lanes_min<LPR>(best.v == bv ? best.i : kNoId)};
             if (writes) {
                 o.top_ids[pos * s.top + k] = top_id(best, said);
                 o.top_log_prob[pos * s.top + k] = top_value(s, best, said);
@@ -193,23 +221,35 @@ constexpr int kLongPacks = 4;               // packs a thread of a long row has 
 constexpr int kCandidates = kThreads * 8 + SSMAP_MAX_TOP;   // one gathering step's most, and the best so far
 
 // A block's alternatives: candidates in any order (their keys differ, so the order of the atomics does not
-// matter), ranked by counting.
+// matter), ranked by counting.  The counting loops read eight keys before they compare: one at a time, each
+// comparison would wait for its own read.
 struct Candidates {
-    Best list[kCandidates];
-    Best kept[SSMAP_MAX_TOP];
+    Key list[kCandidates];
+    Key kept[SSMAP_MAX_TOP];
     int count;
 };
-__device__ __forceinline__ void offer(Candidates &c, const Best &v) { c.list[atomicAdd(&c.count, 1)] = v; }
+__device__ __forceinline__ void offer(Candidates &c, Key k) { c.list[atomicAdd(&c.count, 1)] = k; }
+__device__ __forceinline__ int count_above(const Key *list, int n, Key mine) {
+    int rank = 0, q = 0;
+    for (; q + 8 <= n; q += 8) {
+        Key k[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) k[e] = list[q + e];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) rank += k[e] > mine;
+    }
+    for (; q < n; ++q) rank += list[q] > mine;
+    return rank;
+}
 // The best `top` of the list into kept[], in order; all threads call it.
 __device__ __forceinline__ void rank_candidates(Candidates &c, int top) {
     __syncthreads();
     const int n = c.count;
-    if (threadIdx.x < top) c.kept[threadIdx.x] = Best{-INFINITY, kNoId};
+    if (threadIdx.x < top) c.kept[threadIdx.x] = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += kThreads) {
-        const Best v = c.list[i];
-        int rank = 0;
-        for (int q = 0; q < n; ++q) rank += better(c.list[q], v);
+        const Key v = c.list[i];
+        const int rank = count_above(c.list, n, v);
         if (rank < top) c.kept[rank] = v;
     }
     __syncthreads();
@@ -230,7 +270,7 @@ template <int DT>
 __global__ __launch_bounds__(kThreads) void k_scores_long(Shape s, const elem_t<DT> *logits, const void *ids, Out o, int splits, int64_t segment, char *parts, int64_t part_bytes) {
     constexpr int VEC = 16 / sizeof(elem_t<DT>), U = kLongPacks, STEP = kThreads * VEC;
     __shared__ Sums joint[kThreads / 64];
-    __shared__ Best firsts[kThreads];
+    __shared__ Key firsts[kThreads];
     __shared__ int chosen[SSMAP_MAX_TOP];
     __shared__ Candidates cand;
     const int tid = threadIdx.x;
@@ -248,8 +288,15 @@ __global__ __launch_bounds__(kThreads) void k_scores_long(Shape s, const elem_t<
                 for (int e = 0; e < VEC; ++e) x[e] = j + e < to ? Elem<DT>::get(row[j + e]) : -INFINITY;
             }
         };
+        int64_t id = 0;
+        float xid = 0.0f;
+        if (splits == 1) {   // on their way during the pass
+            id = load_id(s, ids, b, r);
+            if (id >= 0 && id < s.classes) xid = Elem<DT>::get(row[id]);
+        }
         Sums v{-INFINITY, 0.0f, 0.0f};
-        Best first{-INFINITY, (int32_t)(from + tid * VEC)};
+        float first_v = -INFINITY;
+        int32_t first_j = (int32_t)(from + tid * VEC);
         for (int64_t j0 = from + tid * VEC; j0 < to; j0 += U * STEP) {
             float x[U][VEC];
 #pragma unroll
@@ -259,7 +306,7 @@ __global__ __launch_bounds__(kThreads) void k_scores_long(Shape s, const elem_t<
                 float pm = x[u][0];
 #pragma unroll
                 for (int e = 1; e < VEC; ++e) pm = fmaxf(pm, x[u][e]);
-                if (pm > first.v) first = Best{pm, (int32_t)(j0 + u * STEP)};
+                if (pm > first_v) first_v = pm, first_j = (int32_t)(j0 + u * STEP);
                 const float m = fmaxf(v.m, pm), ms = m == -INFINITY ? 0.0f : m;
                 const float d = fmaxf((v.m - ms) * s.scale, kTiny), f = __builtin_amdgcn_exp2f(d);
                 v.wsum = f * (v.wsum + v.sum * d);
@@ -276,17 +323,18 @@ __global__ __launch_bounds__(kThreads) void k_scores_long(Shape s, const elem_t<
         v = lanes_join<64>(s, v);
         __syncthreads();
         if (tid % 64 == 0) joint[tid / 64] = v;
+        const Key first = key_of(first_v, first_j);
         firsts[tid] = first;
         if (!tid) cand.count = 0;
         __syncthreads();
         v = joint[0];
+#pragma unroll
         for (int w = 1; w < kThreads / 64; ++w) v = join(s, v, joint[w]);
         if (s.top) {
-            int rank = 0;
-            for (int q = 0; q < kThreads; ++q) rank += better(firsts[q], first);
+            const int rank = count_above(firsts, kThreads, first);
             if (rank < s.top) chosen[rank] = tid;
             __syncthreads();
-            const Best least = firsts[chosen[s.top - 1]];
+            const Best least = best_of(firsts[chosen[s.top - 1]]);
             const int64_t packs = (to - from + STEP - 1) / STEP, items = packs * s.top;
             for (int64_t i0 = 0; i0 < items; i0 += kThreads) {
                 const int have = cand.count;
@@ -304,7 +352,7 @@ __global__ __launch_bounds__(kThreads) void k_scores_long(Shape s, const elem_t<
                     fetch(j, x);
 #pragma unroll
                     for (int e = 0; e < VEC; ++e)
-                        if (x[e] > -INFINITY && (x[e] > least.v || (x[e] == least.v && j + e < least.i + VEC))) offer(cand, Best{x[e], (int32_t)(j + e)});
+                        if (x[e] > -INFINITY && (x[e] > least.v || (x[e] == least.v && j + e < least.i + VEC))) offer(cand, key_of(x[e], (int32_t)(j + e)));
                 }
                 __syncthreads();
             }
@@ -313,15 +361,14 @@ __global__ __launch_bounds__(kThreads) void k_scores_long(Shape s, const elem_t<
         if (splits > 1) {
             char *part = parts + unit * part_bytes;
             if (!tid) reinterpret_cast<Part *>(part)->sums = v;
-            if (tid < s.top) reinterpret_cast<Best *>(part + sizeof(Part))[tid] = cand.kept[tid];
+            if (tid < s.top) reinterpret_cast<Key *>(part + sizeof(Part))[tid] = cand.kept[tid];
         } else {
-            const int64_t id = load_id(s, ids, b, r);
-            const float xid = id >= 0 && id < s.classes ? Elem<DT>::get(row[id]) : 0.0f;
             const Said said = say(s, v.m, v.sum, v.wsum, id, xid);
             if (!tid) put(o, pos, said);
             if (tid < s.top) {
-                o.top_ids[pos * s.top + tid] = top_id(cand.kept[tid], said);
-                o.top_log_prob[pos * s.top + tid] = top_value(s, cand.kept[tid], said);
+                const Best w = best_of(cand.kept[tid]);
+                o.top_ids[pos * s.top + tid] = top_id(w, said);
+                o.top_log_prob[pos * s.top + tid] = top_value(s, w, said);
             }
         }
     }
@@ -332,15 +379,18 @@ __global__ __launch_bounds__(kThreads) void k_scores_long(Shape s, const elem_t<
 template <int DT>
 __global__ __launch_bounds__(kThreads) void k_scores_join(Shape s, const elem_t<DT> *logits, const void *ids, Out o, int splits, const char *parts, int64_t part_bytes) {
     __shared__ Sums joint[kThreads / 64];
-    __shared__ Best firsts[kThreads], least;
+    __shared__ Key firsts[kThreads], least;
     __shared__ Candidates cand;
     const int tid = threadIdx.x;
     for (int64_t pos = blockIdx.x; pos < s.batch * s.rows; pos += gridDim.x) {
         const int64_t b = pos / s.rows, r = pos % s.rows;
+        const elem_t<DT> *row = logits + b * s.batch_stride + r * s.row_stride;
+        const int64_t id = load_id(s, ids, b, r);
+        const float xid = id >= 0 && id < s.classes ? Elem<DT>::get(row[id]) : 0.0f;
         const char *part = parts + (pos * splits + (tid < splits ? tid : 0)) * part_bytes;
-        const Best *list = reinterpret_cast<const Best *>(part + sizeof(Part));
+        const Key *list = reinterpret_cast<const Key *>(part + sizeof(Part));
         Sums v{-INFINITY, 0.0f, 0.0f};
-        Best first{-INFINITY, kNoId};
+        Key first = 0;
         if (tid < splits) {
             v = reinterpret_cast<const Part *>(part)->sums;
             if (s.top) first = list[0];
@@ -349,31 +399,29 @@ __global__ __launch_bounds__(kThreads) void k_scores_join(Shape s, const elem_t<
         __syncthreads();
         if (tid % 64 == 0) joint[tid / 64] = v;
         firsts[tid] = first;
-        if (!tid) cand.count = 0, least = Best{-INFINITY, kNoId};
+        if (!tid) cand.count = 0, least = 0;
         __syncthreads();
         v = joint[0];
+#pragma unroll
         for (int w = 1; w < kThreads / 64; ++w) v = join(s, v, joint[w]);
         if (s.top) {
-            int rank = 0;
-            for (int q = 0; q < splits; ++q) rank += better(firsts[q], first);
-            if (tid < splits && rank == s.top - 1 && first.v > -INFINITY) least = first;
+            const int rank = count_above(firsts, splits, first);
+            if (first && rank == s.top - 1) least = first;
             __syncthreads();
-            if (tid < splits && rank < s.top)
+            if (first && rank < s.top)
                 for (int k = 0; k < s.top; ++k) {
-                    const Best c = list[k];
-                    if (!(c.v > -INFINITY) || better(least, c)) break;
+                    const Key c = list[k];
+                    if (!c || c < least) break;
                     offer(cand, c);
                 }
             rank_candidates(cand, s.top);
         }
-        const elem_t<DT> *row = logits + b * s.batch_stride + r * s.row_stride;
-        const int64_t id = load_id(s, ids, b, r);
-        const float xid = id >= 0 && id < s.classes ? Elem<DT>::get(row[id]) : 0.0f;
         const Said said = say(s, v.m, v.sum, v.wsum, id, xid);
         if (!tid) put(o, pos, said);
         if (tid < s.top) {
-            o.top_ids[pos * s.top + tid] = top_id(cand.kept[tid], said);
-            o.top_log_prob[pos * s.top + tid] = top_value(s, cand.kept[tid], said);
+            const Best w = best_of(cand.kept[tid]);
+            o.top_ids[pos * s.top + tid] = top_id(w, said);
+            o.top_log_prob[pos * s.top + tid] = top_value(s, w, said);
         }
     }
 }
@@ -386,7 +434,7 @@ struct Split {
 };
 inline Split split_rows(const Shape &s, int dtype) {
     const int64_t n = s.batch * s.rows, step = kThreads * (16 / head_dtype_size(dtype));
-    Split w{1, s.classes, (int64_t)(sizeof(Part) + s.top * sizeof(Best))};
+    Split w{1, s.classes, (int64_t)(sizeof(Part) + s.top * sizeof(Key))};
     if (n == 0 || n >= 512 || s.classes <= step) return w;
     int64_t most = (s.classes + step - 1) / step;
     most = most < 1024 / n ? most : 1024 / n;
@@ -721,7 +769,11 @@ void launch_scores(const Shape &s, const ssmap_log_probs_args &a, hipStream_t st
         k_scores_short<DT, lpr.value, np.value><<<(unsigned)(blocks < kMostBlocks ? blocks : kMostBlocks), kThreads, 0, st>>>(s, x, a.ids, o);
     };
     if (s.classes <= 16 * VEC) return brief(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
-    if (s.classes <= 16 * VEC * NP) return brief(std::integral_constant<int, 16>{}, std::integral_constant<int, NP>{});
+    if (s.classes <= 32 * VEC) return brief(std::integral_constant<int, 16>{}, std::integral_constant<int, 2>{});
+    if constexpr (NP == 4) {
+        if (s.classes <= 48 * VEC) return brief(std::integral_constant<int, 16>{}, std::integral_constant<int, 3>{});
+        if (s.classes <= 64 * VEC) return brief(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
+    }
     if (s.classes <= 64 * VEC * NP) return brief(std::integral_constant<int, 64>{}, std::integral_constant<int, NP>{});
     const Split w = split_rows(s, DT);
     char *parts = static_cast<char *>(a.workspace);
