@@ -105,6 +105,20 @@ __device__ __forceinline__ Pack<DT, N> load_pack(const elem_t<DT> *p) {
 template <int DT, int N>
 __device__ __forceinline__ void store_pack(elem_t<DT> *p, const Pack<DT, N> &r) { __builtin_memcpy(p, &r, sizeof r); }
 
+// The pack at class j of a row that ends at `to`; -inf beyond.  Kept in memory's type: a conversion next to
+// the load would wait for it, and with it every later load.
+template <int DT, int N>
+__device__ __forceinline__ Pack<DT, N> fetch_pack(const elem_t<DT> *row, int64_t j, int64_t to) {
+    if (j + N <= to) return load_pack<DT, N>(row + j);
+    Pack<DT, N> r;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        r.v[e] = Elem<DT>::put(-INFINITY);
+        if (j + e < to) r.v[e] = row[j + e];
+    }
+    return r;
+}
+
 // Running sums of a set of classes relative to its own maximum.
 struct Sums {
     float m, sum, wsum;
@@ -161,25 +175,19 @@ __global__ __launch_bounds__(kThreads) void k_scores_short(Shape s, const elem_t
         const int64_t b = pos / s.rows, r = pos % s.rows;
         const elem_t<DT> *row = logits + b * s.batch_stride + r * s.row_stride;
         float x[NP][VEC];
+        Pack<DT, VEC> in[NP];
 #pragma unroll
-        for (int u = 0; u < NP; ++u) {
-            const int64_t j = (u * LPR + sub) * VEC;
-            if (j + VEC <= s.classes) {
-                const Pack<DT, VEC> v = load_pack<DT, VEC>(row + j);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) x[u][e] = Elem<DT>::get(v.v[e]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) x[u][e] = j + e < s.classes ? Elem<DT>::get(row[j + e]) : -INFINITY;
-            }
-        }
+        for (int u = 0; u < NP; ++u) in[u] = fetch_pack<DT, VEC>(row, (u * LPR + sub) * VEC, s.classes);
         const int64_t id = load_id(s, ids, b, r);
         const float xid = id >= 0 && id < s.classes ? Elem<DT>::get(row[id]) : 0.0f;
         float m = -INFINITY;
 #pragma unroll
         for (int u = 0; u < NP; ++u)
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) m = fmaxf(m, x[u][e]);
+            for (int e = 0; e < VEC; ++e) {
+                x[u][e] = Elem<DT>::get(in[u].v[e]);
+                m = fmaxf(m, x[u][e]);
+            }
         m = lanes_max<LPR>(m);
         const float ms = m == -INFINITY ? 0.0f : m;
         float sum = 0.0f, wsum = 0.0f;
@@ -278,16 +286,6 @@ __global__ __launch_bounds__(kThreads) void k_scores_long(Shape s, const elem_t<
         const int64_t pos = unit / splits, b = pos / s.rows, r = pos % s.rows;
         const int64_t from = unit % splits * segment, to = from + segment < s.classes ? from + segment : s.classes;
         const elem_t<DT> *row = logits + b * s.batch_stride + r * s.row_stride;
-        const auto fetch = [&](int64_t j, float (&x)[VEC]) {
-            if (j + VEC <= to) {
-                const Pack<DT, VEC> v = load_pack<DT, VEC>(row + j);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) x[e] = Elem<DT>::get(v.v[e]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) x[e] = j + e < to ? Elem<DT>::get(row[j + e]) : -INFINITY;
-            }
-        };
         int64_t id = 0;
         float xid = 0.0f;
         if (splits == 1) {   // on their way during the pass
@@ -297,28 +295,41 @@ __global__ __launch_bounds__(kThreads) void k_scores_long(Shape s, const elem_t<
         Sums v{-INFINITY, 0.0f, 0.0f};
         float first_v = -INFINITY;
         int32_t first_j = (int32_t)(from + tid * VEC);
-        for (int64_t j0 = from + tid * VEC; j0 < to; j0 += U * STEP) {
-            float x[U][VEC];
+        const auto take = [&](const Pack<DT, VEC> &in, int64_t j) {
+            float x[VEC], pm = -INFINITY;
 #pragma unroll
-            for (int u = 0; u < U; ++u) fetch(j0 + u * STEP, x[u]);
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                float pm = x[u][0];
-#pragma unroll
-                for (int e = 1; e < VEC; ++e) pm = fmaxf(pm, x[u][e]);
-                if (pm > first_v) first_v = pm, first_j = (int32_t)(j0 + u * STEP);
-                const float m = fmaxf(v.m, pm), ms = m == -INFINITY ? 0.0f : m;
-                const float d = fmaxf((v.m - ms) * s.scale, kTiny), f = __builtin_amdgcn_exp2f(d);
-                v.wsum = f * (v.wsum + v.sum * d);
-                v.sum *= f;
-                v.m = m;
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const float t = (x[u][e] - ms) * s.scale, p = __builtin_amdgcn_exp2f(t);
-                    v.sum += p;
-                    v.wsum += p * fmaxf(t, kTiny);
-                }
+            for (int e = 0; e < VEC; ++e) {
+                x[e] = Elem<DT>::get(in.v[e]);
+                pm = fmaxf(pm, x[e]);
             }
+            if (pm > first_v) first_v = pm, first_j = (int32_t)j;
+            const float m = fmaxf(v.m, pm), ms = m == -INFINITY ? 0.0f : m;
+            const float d = fmaxf((v.m - ms) * s.scale, kTiny), f = __builtin_amdgcn_exp2f(d);
+            v.wsum = f * (v.wsum + v.sum * d);
+            v.sum *= f;
+            v.m = m;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float t = (x[e] - ms) * s.scale, p = __builtin_amdgcn_exp2f(t);
+                v.sum += p;
+                v.wsum += p * fmaxf(t, kTiny);
+            }
+        };
+        int64_t j0 = from;
+        for (; j0 + U * STEP <= to; j0 += U * STEP) {
+            Pack<DT, VEC> in[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) in[u] = load_pack<DT, VEC>(row + j0 + u * STEP + tid * VEC);
+#pragma unroll
+            for (int u = 0; u < U; ++u) take(in[u], j0 + u * STEP + tid * VEC);
+        }
+        if (j0 < to) {
+            Pack<DT, VEC> in[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) in[u] = fetch_pack<DT, VEC>(row, j0 + u * STEP + tid * VEC, to);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (j0 + u * STEP < to) take(in[u], j0 + u * STEP + tid * VEC);
         }
         v = lanes_join<64>(s, v);
         __syncthreads();
@@ -348,11 +359,12 @@ __global__ __launch_bounds__(kThreads) void k_scores_long(Shape s, const elem_t<
                 const int64_t i = i0 + tid;
                 if (i < items) {
                     const int64_t j = from + (i / s.top * kThreads + chosen[i % s.top]) * VEC;
-                    float x[VEC];
-                    fetch(j, x);
+                    const Pack<DT, VEC> in = fetch_pack<DT, VEC>(row, j, to);
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e)
-                        if (x[e] > -INFINITY && (x[e] > least.v || (x[e] == least.v && j + e < least.i + VEC))) offer(cand, key_of(x[e], (int32_t)(j + e)));
+                    for (int e = 0; e < VEC; ++e) {
+                        const float x = Elem<DT>::get(in.v[e]);
+                        if (x > -INFINITY && (x > least.v || (x == least.v && j + e < least.i + VEC))) offer(cand, key_of(x, (int32_t)(j + e)));
+                    }
                 }
                 __syncthreads();
             }
