@@ -105,16 +105,16 @@ __device__ __forceinline__ Pack<DT, N> load_pack(const elem_t<DT> *p) {
 template <int DT, int N>
 __device__ __forceinline__ void store_pack(elem_t<DT> *p, const Pack<DT, N> &r) { __builtin_memcpy(p, &r, sizeof r); }
 
-// The pack at class j of a row that ends at `to`; -inf beyond.  Kept in memory's type: a conversion next to
-// the load would wait for it, and with it every later load.
+// The pack at class j of a row, of which classes from ... to - 1 may be read; -inf for the others.  Kept in
+// memory's type: a conversion next to the load would wait for it, and with it every later load.
 template <int DT, int N>
-__device__ __forceinline__ Pack<DT, N> fetch_pack(const elem_t<DT> *row, int64_t j, int64_t to) {
-    if (j + N <= to) return load_pack<DT, N>(row + j);
+__device__ __forceinline__ Pack<DT, N> fetch_pack(const elem_t<DT> *row, int j, int from, int to) {
+    if (j >= from && j + N <= to) return load_pack<DT, N>(row + j);
     Pack<DT, N> r;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
         r.v[e] = Elem<DT>::put(-INFINITY);
-        if (j + e < to) r.v[e] = row[j + e];
+        if (j + e >= from && j + e < to) r.v[e] = row[j + e];
     }
     return r;
 }
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(kThreads) void k_scores_short(Shape s, const elem_t
         float x[NP][VEC];
         Pack<DT, VEC> in[NP];
 #pragma unroll
-        for (int u = 0; u < NP; ++u) in[u] = fetch_pack<DT, VEC>(row, (u * LPR + sub) * VEC, s.classes);
+        for (int u = 0; u < NP; ++u) in[u] = fetch_pack<DT, VEC>(row, (u * LPR + sub) * VEC, 0, (int)s.classes);
         const int64_t id = load_id(s, ids, b, r);
         const float xid = id >= 0 && id < s.classes ? Elem<DT>::get(row[id]) : 0.0f;
         float m = -INFINITY;
@@ -225,8 +225,10 @@ __global__ __launch_bounds__(kThreads) void k_scores_short(Shape s, const elem_t
     }
 }
 
-constexpr int kLongPacks = 4;               // packs a thread of a long row has in flight
-constexpr int kCandidates = kThreads * 8 + SSMAP_MAX_TOP;   // one gathering step's most, and the best so far
+constexpr int kLongPacks = 2;               // packs a thread of a long row has in flight: one step
+constexpr int kSteps = 16;                  // what a thread remembers the maxima of
+constexpr int kGathered = 1024;             // logits looked at again in one go
+constexpr int kCandidates = kGathered + SSMAP_MAX_TOP;
 
 // A block's alternatives: candidates in any order (their keys differ, so the order of the atomics does not
 // matter), ranked by counting.  The counting loops read eight keys before they compare: one at a time, each
@@ -268,41 +270,51 @@ struct Part {       // what a segment of a split row says, followed by `top` alt
     float pad;
 };
 
-// Long rows: a block takes one segment of a row, in one pass over memory.  Each thread keeps running sums of
-// its packs (rescaled once a pack) and where its largest logit first stood.  At the end the `top` threads
-// with the best maxima hold every alternative: any other thread's logits are beaten by those `top` maxima
-// (values first; among equal ones the thread whose pack comes first wins, and its pack lies in front of the
-// other's).  Only their packs are read again, from the caches, and only what is at least the last of the
-// maxima becomes a candidate.
+// Long rows: a block takes one segment of a row, in one pass over memory.  Packs lie at addresses that are
+// multiples of 16 whatever the row's start (loads that straddle such addresses cost 14 of 78 us at 4096 x
+// 32003 fp16); the first and last are masked.  Each thread keeps running sums of its packs (rescaled once a
+// pack), where its largest logit first stood, and the upper 16 bits of the maxima of up to kSteps stretches.
+//
+// Alternatives: the `top` threads with the best maxima hold them all.  Any other thread's logits are beaten by
+// those `top` maxima: by value first; among equal ones the thread whose pack comes first wins, and its pack
+// lies in front of the other's.  The threshold that `top` of the 256 keys pass is found bit by bit with
+// ballots, every wave by itself (counting for each key the keys above it kept the LDS busy for 10 us of 78).
+// Of the chosen threads only the stretches whose maximum reaches the threshold are read again, from the
+// caches, and only logits that reach it become candidates.
 template <int DT>
-__global__ __launch_bounds__(kThreads) void k_scores_long(Shape s, const elem_t<DT> *logits, const void *ids, Out o, int splits, int64_t segment, char *parts, int64_t part_bytes) {
+__global__ __launch_bounds__(kThreads, 8) void k_scores_long(Shape s, const elem_t<DT> *logits, const void *ids, Out o, int splits, int64_t segment, char *parts, int64_t part_bytes) {
     constexpr int VEC = 16 / sizeof(elem_t<DT>), U = kLongPacks, STEP = kThreads * VEC;
     __shared__ Sums joint[kThreads / 64];
     __shared__ Key firsts[kThreads];
-    __shared__ int chosen[SSMAP_MAX_TOP];
+    __shared__ uint16_t steps[kSteps][kThreads], items[kSteps * SSMAP_MAX_TOP];
+    __shared__ int n_chosen, n_items;
+    __shared__ uint8_t chosen[SSMAP_MAX_TOP];
     __shared__ Candidates cand;
     const int tid = threadIdx.x;
     for (int64_t unit = blockIdx.x; unit < s.batch * s.rows * splits; unit += gridDim.x) {
         const int64_t pos = unit / splits, b = pos / s.rows, r = pos % s.rows;
-        const int64_t from = unit % splits * segment, to = from + segment < s.classes ? from + segment : s.classes;
+        const int from = (int)(unit % splits * segment), to = (int)(from + segment < s.classes ? from + segment : s.classes);   // classes <= 2^30
         const elem_t<DT> *row = logits + b * s.batch_stride + r * s.row_stride;
+        const int lo = from - (int)(reinterpret_cast<uintptr_t>(row + from) % 16 / sizeof(elem_t<DT>));
         int64_t id = 0;
         float xid = 0.0f;
         if (splits == 1) {   // on their way during the pass
             id = load_id(s, ids, b, r);
             if (id >= 0 && id < s.classes) xid = Elem<DT>::get(row[id]);
         }
+        const int n_steps = (to - lo + U * STEP - 1) / (U * STEP), per = (n_steps + kSteps - 1) / kSteps;
         Sums v{-INFINITY, 0.0f, 0.0f};
-        float first_v = -INFINITY;
-        int32_t first_j = (int32_t)(from + tid * VEC);
-        const auto take = [&](const Pack<DT, VEC> &in, int64_t j) {
+        float first_v = -INFINITY, stretch = -INFINITY;
+        int first_j = from + tid * VEC;
+        const auto take = [&](const Pack<DT, VEC> &in, int j) {
             float x[VEC], pm = -INFINITY;
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 x[e] = Elem<DT>::get(in.v[e]);
                 pm = fmaxf(pm, x[e]);
             }
-            if (pm > first_v) first_v = pm, first_j = (int32_t)j;
+            if (pm > first_v) first_v = pm, first_j = j > from ? j : from;
+            stretch = fmaxf(stretch, pm);
             const float m = fmaxf(v.m, pm), ms = m == -INFINITY ? 0.0f : m;
             const float d = fmaxf((v.m - ms) * s.scale, kTiny), f = __builtin_amdgcn_exp2f(d);
             v.wsum = f * (v.wsum + v.sum * d);
@@ -315,55 +327,70 @@ __global__ __launch_bounds__(kThreads) void k_scores_long(Shape s, const elem_t<
                 v.wsum += p * fmaxf(t, kTiny);
             }
         };
-        int64_t j0 = from;
-        for (; j0 + U * STEP <= to; j0 += U * STEP) {
+        for (int step = 0; step < n_steps; ++step) {
+            const int j0 = lo + step * (U * STEP), j = j0 + tid * VEC;
             Pack<DT, VEC> in[U];
+            if ((step || lo == from) && j0 + U * STEP <= to) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) in[u] = load_pack<DT, VEC>(row + j0 + u * STEP + tid * VEC);
+                for (int u = 0; u < U; ++u) in[u] = load_pack<DT, VEC>(row + j + u * STEP);
+            } else {
 #pragma unroll
-            for (int u = 0; u < U; ++u) take(in[u], j0 + u * STEP + tid * VEC);
+                for (int u = 0; u < U; ++u) in[u] = fetch_pack<DT, VEC>(row, j + u * STEP, from, to);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) take(in[u], j + u * STEP);
+            if (s.top && (step + 1) % per == 0) steps[step / per][tid] = (uint16_t)(key_of(stretch, 0) >> 48), stretch = -INFINITY;
         }
-        if (j0 < to) {
-            Pack<DT, VEC> in[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) in[u] = fetch_pack<DT, VEC>(row, j0 + u * STEP + tid * VEC, to);
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (j0 + u * STEP < to) take(in[u], j0 + u * STEP + tid * VEC);
-        }
+        if (s.top && n_steps % per) steps[n_steps / per][tid] = (uint16_t)(key_of(stretch, 0) >> 48);
         v = lanes_join<64>(s, v);
         __syncthreads();
         if (tid % 64 == 0) joint[tid / 64] = v;
         const Key first = key_of(first_v, first_j);
         firsts[tid] = first;
-        if (!tid) cand.count = 0;
+        if (!tid) cand.count = n_chosen = n_items = 0;
         __syncthreads();
         v = joint[0];
 #pragma unroll
         for (int w = 1; w < kThreads / 64; ++w) v = join(s, v, joint[w]);
         if (s.top) {
-            const int rank = count_above(firsts, kThreads, first);
-            if (rank < s.top) chosen[rank] = tid;
+            Key all[kThreads / 64], least = 0;
+#pragma unroll
+            for (int q = 0; q < kThreads / 64; ++q) all[q] = firsts[q * 64 + tid % 64];
+            for (int bit = 63; bit >= 0; --bit) {
+                const Key t = least | (Key)1 << bit;
+                int n = 0;
+#pragma unroll
+                for (int q = 0; q < kThreads / 64; ++q) n += __popcll(__ballot(all[q] >= t));
+                if (n >= s.top) least = t;
+                if (n == s.top) break;
+            }
+            if (first >= least) chosen[atomicAdd(&n_chosen, 1)] = (uint8_t)tid;   // exactly `top` threads
             __syncthreads();
-            const Best least = best_of(firsts[chosen[s.top - 1]]);
-            const int64_t packs = (to - from + STEP - 1) / STEP, items = packs * s.top;
-            for (int64_t i0 = 0; i0 < items; i0 += kThreads) {
+            for (int i = tid; i < s.top * kSteps; i += kThreads) {
+                const int th = chosen[i / kSteps], st = i % kSteps;
+                if (st * per < n_steps && steps[st][th] >= (uint16_t)(least >> 48)) items[atomicAdd(&n_items, 1)] = (uint16_t)(st * kThreads + th);
+            }
+            __syncthreads();
+            const int packs = per * U, all_packs = n_items * packs;
+            for (int p0 = 0; p0 < all_packs; p0 += kGathered / VEC) {
                 const int have = cand.count;
                 __syncthreads();   // nobody offers before everybody has read the count
-                if (have > kCandidates - kThreads * VEC) {
+                if (have > kCandidates - kGathered) {
                     rank_candidates(cand, s.top);
                     if (tid < s.top) cand.list[tid] = cand.kept[tid];
                     if (!tid) cand.count = s.top;
                     __syncthreads();
                 }
-                const int64_t i = i0 + tid;
-                if (i < items) {
-                    const int64_t j = from + (i / s.top * kThreads + chosen[i % s.top]) * VEC;
-                    const Pack<DT, VEC> in = fetch_pack<DT, VEC>(row, j, to);
+                const int p = p0 + tid;
+                if (tid < kGathered / VEC && p < all_packs) {
+                    const int item = items[p / packs];
+                    const int j = lo + ((item / kThreads * packs + p % packs) * kThreads + item % kThreads) * VEC;
+                    const Pack<DT, VEC> in = fetch_pack<DT, VEC>(row, j, from, to);
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) {
+                    for (int e = 0; e < VEC; ++e) {   // a thread's key stands at its pack's start
                         const float x = Elem<DT>::get(in.v[e]);
-                        if (x > -INFINITY && (x > least.v || (x == least.v && j + e < least.i + VEC))) offer(cand, key_of(x, (int32_t)(j + e)));
+                        const Key k = key_of(x, j + e);
+                        if (x > -INFINITY && k + (VEC - 1) >= least) offer(cand, k);
                     }
                 }
                 __syncthreads();
