@@ -162,24 +162,37 @@ __device__ __forceinline__ Sums lanes_join(const Shape &s, Sums v) {
     return {m, lanes_sum<LANES>(f * v.sum), lanes_sum<LANES>(f * (v.wsum + v.sum * dv))};
 }
 
+constexpr int kShortBlocks = 256 * 6;   // as many as are resident at once: each block loops over rows
+
 // Short rows: LPR lanes hold a row in registers (NP packs a lane), so the maximum is known before the sums
 // and each alternative is found by one more look at the registers.
 template <int DT, int LPR, int NP>
 __global__ __launch_bounds__(kThreads) void k_scores_short(Shape s, const elem_t<DT> *logits, const void *ids, Out o) {
     constexpr int VEC = 16 / sizeof(elem_t<DT>), UNITS = kThreads / LPR;
     const int sub = threadIdx.x % LPR;
-    const int64_t n = s.batch * s.rows;
-    // every lane stays in the loop as long as its block has a row: the exchanges below need all of a wave
-    for (int64_t first = blockIdx.x * (int64_t)UNITS; first < n; first += (int64_t)gridDim.x * UNITS) {
+    const int64_t n = s.batch * s.rows, stride = (int64_t)gridDim.x * UNITS;
+    const auto place = [&](int64_t first, int64_t &b, int64_t &r) {   // lanes behind the last row take that one again
         const int64_t mine = first + threadIdx.x / LPR, pos = mine < n ? mine : n - 1;
-        const int64_t b = pos / s.rows, r = pos % s.rows;
+        b = pos / s.rows, r = pos % s.rows;
+        return pos;
+    };
+    const auto fetch = [&](int64_t b, int64_t r, Pack<DT, VEC> (&in)[NP], int64_t &id) {
         const elem_t<DT> *row = logits + b * s.batch_stride + r * s.row_stride;
-        float x[NP][VEC];
-        Pack<DT, VEC> in[NP];
+        id = load_id(s, ids, b, r);
 #pragma unroll
         for (int u = 0; u < NP; ++u) in[u] = fetch_pack<DT, VEC>(row, (u * LPR + sub) * VEC, 0, (int)s.classes);
-        const int64_t id = load_id(s, ids, b, r);
+    };
+    Pack<DT, VEC> in[NP], next[NP];
+    int64_t b, r, id, b2, r2, id2 = 0, pos = place(blockIdx.x * (int64_t)UNITS, b, r), pos2;
+    fetch(b, r, in, id);
+    // every lane stays in the loop as long as its block has a row: the exchanges below need all of a wave
+    for (int64_t first = blockIdx.x * (int64_t)UNITS; first < n; first += stride) {
+        const bool mine = first + threadIdx.x / LPR < n;
+        const elem_t<DT> *row = logits + b * s.batch_stride + r * s.row_stride;
         const float xid = id >= 0 && id < s.classes ? Elem<DT>::get(row[id]) : 0.0f;
+        pos2 = place(first + stride, b2, r2);
+        if (first + stride < n) fetch(b2, r2, next, id2);   // the next row is under way while this one is worked on
+        float x[NP][VEC];
         float m = -INFINITY;
 #pragma unroll
         for (int u = 0; u < NP; ++u)
@@ -202,7 +215,7 @@ __global__ __launch_bounds__(kThreads) void k_scores_short(Shape s, const elem_t
         sum = lanes_sum<LPR>(sum);
         wsum = lanes_sum<LPR>(wsum);
         const Said said = say(s, m, sum, wsum, id, xid);
-        const bool writes = sub == 0 && mine < n;
+        const bool writes = sub == 0 && mine;
         if (writes) put(o, pos, said);
         Best last{INFINITY, -1};
         for (int k = 0; k < s.top; ++k) {
@@ -222,6 +235,9 @@ __global__ __launch_bounds__(kThreads) void k_scores_short(Shape s, const elem_t
             }
             last = best;
         }
+        b = b2, r = r2, id = id2, pos = pos2;
+#pragma unroll
+        for (int u = 0; u < NP; ++u) in[u] = next[u];
     }
 }
 
@@ -805,7 +821,7 @@ void launch_scores(const Shape &s, const ssmap_log_probs_args &a, hipStream_t st
     const int64_t n = s.batch * s.rows;
     const auto brief = [&](auto lpr, auto np) {
         const int64_t blocks = (n + kThreads / lpr.value - 1) / (kThreads / lpr.value);
-        k_scores_short<DT, lpr.value, np.value><<<(unsigned)(blocks < kMostBlocks ? blocks : kMostBlocks), kThreads, 0, st>>>(s, x, a.ids, o);
+        k_scores_short<DT, lpr.value, np.value><<<(unsigned)(blocks < kShortBlocks ? blocks : kShortBlocks), kThreads, 0, st>>>(s, x, a.ids, o);
     };
     if (s.classes <= 16 * VEC) return brief(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
     if (s.classes <= 32 * VEC) return brief(std::integral_constant<int, 16>{}, std::integral_constant<int, 2>{});

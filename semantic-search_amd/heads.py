@@ -110,21 +110,19 @@ def _two(name, sizes, *strides):
     return tuple([1] * pad + n), [tuple([0] * pad + s) for s in merged[1:]]
 
 
-def _stream(device):
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-
-
 def _call(device, entry, args, workspace=None):
     """One C call with `device` current; the workspace, if any, is torch's, on the current stream."""
-    with torch.cuda.device(device):
-        if workspace is not None:
-            need = workspace(C.byref(args))
-            if need < 0:
-                _capi.check(1)
-            if need:
-                ws = torch.empty(need, dtype=torch.uint8, device=device)
-                args.workspace, args.workspace_bytes = ws.data_ptr(), need
-        _capi.check(entry(C.byref(args), _stream(device)))
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return _call(device, entry, args, workspace)
+    if workspace is not None:
+        need = workspace(C.byref(args))
+        if need < 0:
+            _capi.check(1)
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=device)
+            args.workspace, args.workspace_bytes = ws.data_ptr(), need
+    _capi.check(entry(C.byref(args), torch._C._cuda_getCurrentRawStream(device.index)))
 
 
 def _score_layout(logits, ids, dim):
