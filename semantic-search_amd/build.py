@@ -26,6 +26,9 @@ SOURCES = [
     ("fuse.hip", []),
     ("scores.hip", []),
     ("linear.hip", []),
+    ("tiles_f32.hip", []),
+    ("tiles_bf16.hip", []),
+    ("tiles_f16.hip", []),
     ("engine.cpp", ["-ffp-contract=off"]),
 ]
 # no packed float32 instructions (v_pk_add_f32, v_pk_mul_f32, v_pk_fma_f32): the compiler makes them from
@@ -46,7 +49,7 @@ def _newer(target, deps):
 def build(force: bool = False, verbose: bool = True) -> str:
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     headers = [os.path.join(CSRC, "ssmap_internal.h"), os.path.join(CSRC, "rows.h"),
-               os.path.join(CSRC, "heads.h"),
+               os.path.join(CSRC, "heads.h"), os.path.join(CSRC, "products.h"), os.path.join(CSRC, "tiles.h"),
                os.path.join(ROOT, "include", "ssmap.h")]
     os.makedirs(LIB_DIR, exist_ok=True)
     os.makedirs(OBJ_DIR, exist_ok=True)

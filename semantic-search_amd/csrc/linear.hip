@@ -7,36 +7,12 @@
 #include <math.h>
 
 #include "heads.h"
+#include "products.h"
+#include "tiles.h"
 
 using namespace ssmap;
 
 namespace {
-
-struct Product {
-    int64_t M, N, K;
-    int64_t out_batches;                    // out, a, b and the epilogue advance together
-    int64_t sum_batches;                    // the sum runs over this many blocks of K as well (planes: over the envs)
-    const void *a, *b;
-    int64_t a_m, a_k, a_out, a_sum;         // strides; of an out batch; of a sum batch
-    int64_t b_n, b_k, b_out, b_sum;
-    void *out;                              // dense [out_batches][M][N]
-    void *pre;                              // the same in the operands' type, or NULL
-    const void *bias, *res;
-    int32_t bias_f32, bias_along_m, act, pad;
-    int64_t res_out, res_m;
-};
-
-__device__ __forceinline__ float activate(float z, int act) {
-    if (act == SSMAP_ACT_RELU) return z < 0.0f ? 0.0f : z;
-    if (act == SSMAP_ACT_GELU) return 0.5f * z * erfcf(-0.70710678118654752f * z);
-    if (act == SSMAP_ACT_GELU_TANH) {
-        // (1 + tanh u) / 2 = 1 / (1 + exp(-2u))
-        const float u = 0.79788456080286536f * (z + 0.044715f * z * z * z);
-        return z / (1.0f + expf(-2.0f * u));
-    }
-    if (act == SSMAP_ACT_SILU) return z / (1.0f + expf(-z));
-    return z;
-}
 
 __device__ __forceinline__ float slope(float z, int act) {
     if (act == SSMAP_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
@@ -53,57 +29,6 @@ __device__ __forceinline__ float slope(float z, int act) {
         return q + (q > 0.0f && q < 1.0f ? z * q * (1.0f - q) : 0.0f);
     }
     return 1.0f;
-}
-
-// One element of the result: `o` is its place in the dense output.
-template <int DT, int OT>
-__device__ __forceinline__ void finish(const Product &p, int64_t o, int64_t e, int64_t m, int64_t n, float z) {
-    if (p.bias) {
-        const int64_t i = p.bias_along_m ? m : n;
-        z += p.bias_f32 ? static_cast<const float *>(p.bias)[i] : Elem<DT>::get(static_cast<const elem_t<DT> *>(p.bias)[i]);
-    }
-    if (p.pre) static_cast<elem_t<DT> *>(p.pre)[o] = Elem<DT>::put(z);
-    z = activate(z, p.act);
-    if (p.res) z += Elem<OT>::get(static_cast<const elem_t<OT> *>(p.res)[e * p.res_out + m * p.res_m + n]);
-    static_cast<elem_t<OT> *>(p.out)[o] = Elem<OT>::put(z);
-}
-
-// 64 x 64 tiles, four by four results a thread.
-template <int DT, int OT>
-__global__ __launch_bounds__(256) void k_product(Product p) {
-    constexpr int T = 64, D = 16;
-    __shared__ float as[D][T + 1], bs[D][T + 1];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int64_t tiles_n = (p.N + T - 1) / T, tiles_m = (p.M + T - 1) / T;
-    for (int64_t tile = blockIdx.x; tile < tiles_m * tiles_n * p.out_batches; tile += gridDim.x) {
-        const int64_t e = tile / (tiles_m * tiles_n), rest = tile % (tiles_m * tiles_n);
-        const int64_t m0 = rest / tiles_n * T, n0 = rest % tiles_n * T;
-        float acc[4][4] = {};
-        for (int64_t sb = 0; sb < p.sum_batches; ++sb) {
-            const elem_t<DT> *a = static_cast<const elem_t<DT> *>(p.a) + e * p.a_out + sb * p.a_sum;
-            const elem_t<DT> *b = static_cast<const elem_t<DT> *>(p.b) + e * p.b_out + sb * p.b_sum;
-            for (int64_t k0 = 0; k0 < p.K; k0 += D) {
-                __syncthreads();
-                for (int i = threadIdx.x; i < T * D; i += 256) {
-                    // neighbouring threads walk whichever axis is dense
-                    const int am = p.a_k == 1 ? i / D : i % T, ak = p.a_k == 1 ? i % D : i / T;
-                    const int bn = p.b_k == 1 ? i / D : i % T, bk = p.b_k == 1 ? i % D : i / T;
-                    as[ak][am] = m0 + am < p.M && k0 + ak < p.K ? Elem<DT>::get(a[(m0 + am) * p.a_m + (k0 + ak) * p.a_k]) : 0.0f;
-                    bs[bk][bn] = n0 + bn < p.N && k0 + bk < p.K ? Elem<DT>::get(b[(n0 + bn) * p.b_n + (k0 + bk) * p.b_k]) : 0.0f;
-                }
-                __syncthreads();
-                for (int k = 0; k < D; ++k)
-                    for (int i = 0; i < 4; ++i)
-                        for (int j = 0; j < 4; ++j) acc[i][j] += as[k][ty * 4 + i] * bs[k][tx + 16 * j];
-            }
-        }
-        for (int i = 0; i < 4; ++i)
-            for (int j = 0; j < 4; ++j) {
-                const int64_t m = m0 + ty * 4 + i, n = n0 + tx + 16 * j;
-                if (m < p.M && n < p.N) finish<DT, OT>(p, (e * p.M + m) * p.N + n, e, m, n, acc[i][j]);
-            }
-        __syncthreads();
-    }
 }
 
 // dz = g act'(pre) in the products' type, dense.  out: [batch][P][Q], g strided by (batch, P).
@@ -141,14 +66,6 @@ __global__ __launch_bounds__(256) void k_bias_grad(int64_t batch, int64_t rows, 
         if (!threadIdx.x) out[n] = Elem<DT>::put(part[0]);
         __syncthreads();
     }
-}
-
-inline unsigned blocks(int64_t n) { return (unsigned)(n < 1 ? 1 : n < (1 << 20) ? n : (1 << 20)); }
-
-template <int DT, int OT>
-void launch_product(const Product &p, hipStream_t st) {
-    const int64_t tiles = (p.M + 63) / 64 * ((p.N + 63) / 64) * p.out_batches;
-    if (tiles) k_product<DT, OT><<<blocks(tiles), 256, 0, st>>>(p);
 }
 
 // Calls f with the operand type and the output's type (the same or float) as constants.

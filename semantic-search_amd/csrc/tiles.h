@@ -1,0 +1,442 @@
+// Matrix products on the matrix cores: out[m][n] = sum_k a(m, k) b(n, k), tile by tile.
+//
+// A block computes BI x BJ results, I the m side and J the n side, dense in memory.  A stage is 128 bytes of
+// every tile row in the sum's direction (64 values of 16 bits, 32 of float32), laid out in LDS as 16-byte
+// chunks; two stages alternate.  A side whose sum direction is dense in memory (KC) keeps its rows: chunk c
+// of row r sits at slot r * 8 + (c ^ (r & 7)), so that the 16 rows that one matrix instruction reads at one
+// c lie in different banks.  A side whose other direction is dense keeps rows of the sum index instead, and
+// is turned while it is read: ds_read_b64_tr_b16 gives lane q of 16 the values of column q from four rows of
+// 16 columns.  Its chunks are swizzled by 32 bytes a row, so that the four rows lie in different banks.
+//
+// The matrix instruction takes J as its rows and I as its columns: a lane then holds four neighbouring n of
+// one m, which the epilogue reads and writes together.
+#pragma once
+
+#include "products.h"
+
+namespace ssmap {
+
+using f32x4 = float __attribute__((ext_vector_type(4)));
+using i32x4 = int __attribute__((ext_vector_type(4)));
+using bf16x8 = __bf16 __attribute__((ext_vector_type(8)));
+using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
+using i16x4 = short __attribute__((ext_vector_type(4)));
+
+// acc += (chunk of J) x (chunk of I): every lane of a group of 16 holds the same stretch of the sum, groups
+// hold neighbouring stretches.
+template <int DT>
+__device__ __forceinline__ f32x4 mma_chunk(i32x4 j, i32x4 i, f32x4 acc) {
+    if constexpr (DT == SSMAP_BF16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, j), __builtin_bit_cast(bf16x8, i), acc, 0, 0, 0);
+    } else if constexpr (DT == SSMAP_F16) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, j), __builtin_bit_cast(f16x8, i), acc, 0, 0, 0);
+    } else {
+        const f32x4 a = __builtin_bit_cast(f32x4, j), b = __builtin_bit_cast(f32x4, i);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], b[s], acc, 0, 0, 0);
+        return acc;
+    }
+}
+
+constexpr uint32_t kNowhere = 0xFFFFFFF0u;   // a buffer offset behind every descriptor's end: reads as zero
+
+// One side of a tile: R rows (or columns) of it, NT threads.
+template <int DT, bool KC, int R, int NT>
+struct Side {
+    static constexpr int SIZE = head_dtype_size(DT), E = 16 / SIZE, KB = 128 / SIZE;   // values a chunk, a stage
+    static constexpr int PER = R * 8 / NT, ROW = R / E;                                // chunks a thread; a row (not KC)
+    static constexpr int BYTES = R * 128;
+    static_assert(R * 8 % NT == 0 && (KC || ROW >= 8), "tile shape");
+
+    static __device__ __forceinline__ int swizzle(int k) { return DT == SSMAP_F32 ? ((k >> 2) & 3) << 2 : (k & 3) << 1; }
+
+    // chunk of slot s: its row (KC) or sum index (not KC), and its place there
+    static __device__ __forceinline__ void place(int s, int &line, int &c) {
+        if constexpr (KC) line = s / 8, c = (s % 8) ^ (line & 7);
+        else line = s / ROW, c = (s % ROW) ^ swizzle(line);
+    }
+    // how many of its values exist: `rows` are left on this side, `ks` in the sum
+    static __device__ __forceinline__ int count(int line, int c, int rows, int ks) {
+        const int across = KC ? rows : ks, along = (KC ? ks : rows) - c * E;
+        return line < across ? (along < 0 ? 0 : along < E ? along : E) : 0;
+    }
+
+    // Straight from memory to LDS: 16 bytes a lane, a wave's 64 chunks land one after the other.  `base` is the
+    // tile's corner, `ld` the bytes of a line; both multiples of 16, and so are the dense extents in bytes.
+    static __device__ __forceinline__ void offsets(uint32_t (&off)[PER], int rows, int ks, uint32_t ld) {
+#pragma unroll
+        for (int it = 0; it < PER; ++it) {
+            int line, c;
+            place(it * NT + threadIdx.x, line, c);
+            off[it] = count(line, c, rows, ks) ? line * ld + c * 16 : kNowhere;
+        }
+    }
+    static __device__ __forceinline__ void fetch(const char *base, const uint32_t (&off)[PER], uint32_t lds) {
+        // word 1 holds the address's upper bits and no stride, word 2 the length, word 3 a raw format
+        const uint64_t at = (uint64_t)base;
+        const i32x4 desc = {(int)(uint32_t)at, (int)(uint32_t)(at >> 32) & 0xFFFF, (int)0x80000000u, 0x00020000};
+        const uint32_t first = lds + (threadIdx.x / 64) * 1024;
+#pragma unroll
+        for (int it = 0; it < PER; ++it) {
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
+                             __builtin_amdgcn_readfirstlane(first + it * NT * 16)),
+                         "v"(off[it]), "s"(desc)
+                         : "memory");
+        }
+    }
+
+    // Through registers, for any alignment and extent.
+    static __device__ __forceinline__ void load(i32x4 (&reg)[PER], const char *base, int rows, int ks, int64_t ld) {
+#pragma unroll
+        for (int it = 0; it < PER; ++it) {
+            int line, c;
+            place(it * NT + threadIdx.x, line, c);
+            const int n = count(line, c, rows, ks);
+            const char *p = base + line * ld + c * 16;
+            i32x4 v = {0, 0, 0, 0};
+            if (n == E) {
+                __builtin_memcpy(&v, p, 16);
+            } else {
+                elem_t<DT> e[E];
+#pragma unroll
+                for (int q = 0; q < E; ++q) {
+                    e[q] = Elem<DT>::put(0.0f);
+                    if (q < n) e[q] = reinterpret_cast<const elem_t<DT> *>(p)[q];
+                }
+                __builtin_memcpy(&v, e, 16);
+            }
+            reg[it] = v;
+        }
+    }
+    static __device__ __forceinline__ void store(const i32x4 (&reg)[PER], char *lds) {
+#pragma unroll
+        for (int it = 0; it < PER; ++it) *reinterpret_cast<i32x4 *>(lds + (it * NT + threadIdx.x) * 16) = reg[it];
+    }
+
+    // The chunk of rows row0 ... row0 + 15 for half kk of the stage.
+    static __device__ __forceinline__ i32x4 read(const char *lds, int row0, int kk) {
+        const int lane = threadIdx.x % 64, q = lane % 16, g = lane / 16;
+        if constexpr (KC) {
+            return *reinterpret_cast<const i32x4 *>(lds + (row0 + q) * 128 + (((kk * 4 + g) ^ (q & 7)) * 16));
+        } else if constexpr (DT == SSMAP_F32) {
+            f32x4 v;
+            const int i = row0 + q;
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const int k = kk * 16 + g * 4 + s;
+                v[s] = *reinterpret_cast<const float *>(lds + (k * ROW + ((i / 4) ^ swizzle(k))) * 16 + (i & 3) * 4);
+            }
+            return __builtin_bit_cast(i32x4, v);
+        } else {
+            union {
+                i16x4 h[2];
+                i32x4 v;
+            } u;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int k = kk * 32 + g * 8 + h * 4 + q / 4;
+                const char *p = lds + (k * ROW + ((row0 / 8 + (q % 4) / 2) ^ swizzle(k))) * 16 + (q & 1) * 8;
+                u.h[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4 *)p);
+            }
+            return u.v;
+        }
+    }
+};
+
+// FINE: for results in float32.  Results of 16 bits take erfc from Abramowitz and Stegun's formula 7.1.26,
+// whose error of 1.5e-7 is far below their rounding.
+template <bool FINE>
+__device__ __forceinline__ float half_erfc(float x) {   // erfc(x) / 2
+    if constexpr (FINE) return 0.5f * erfcf(x);
+    const float a = fabsf(x), t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * a);
+    const float y = t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f))));
+    const float v = y * __builtin_amdgcn_exp2f(-1.44269504088896341f * a * a);
+    return x < 0.0f ? 1.0f - v : v;
+}
+template <bool FINE>
+__device__ __forceinline__ float logistic(float x) {    // 1 / (1 + exp(-x))
+    if constexpr (FINE) return 1.0f / (1.0f + expf(-x));
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * x));
+}
+template <bool FINE>
+__device__ __forceinline__ float activate(float z, int act) {
+    if (act == SSMAP_ACT_RELU) return z < 0.0f ? 0.0f : z;
+    if (act == SSMAP_ACT_GELU) return z * half_erfc<FINE>(-0.70710678118654752f * z);
+    if (act == SSMAP_ACT_GELU_TANH) {
+        // (1 + tanh u) / 2 = 1 / (1 + exp(-2u))
+        return z * logistic<FINE>(1.5957691216057308f * (z + 0.044715f * z * z * z));
+    }
+    if (act == SSMAP_ACT_SILU) return z * logistic<FINE>(z);
+    return z;
+}
+
+// N results next to each other (n, n + 1, ...), of which `left` exist.  `o` is the first one's place in the
+// dense output.
+template <int DT, int OT, int N>
+__device__ __forceinline__ void finish(const Product &p, int64_t o, int64_t e, int64_t m, int64_t n, int left, float (&z)[N]) {
+    const auto each = [&](auto f) {
+#pragma unroll
+        for (int q = 0; q < N; ++q)
+            if (q < left) f(q);
+    };
+    const auto get = [&](auto tag, const void *from, int64_t at, float (&v)[N]) {
+        constexpr int T = decltype(tag)::value;
+        const elem_t<T> *src = static_cast<const elem_t<T> *>(from) + at;
+        if (left >= N) {
+            elem_t<T> w[N];
+            __builtin_memcpy(w, src, sizeof w);
+#pragma unroll
+            for (int q = 0; q < N; ++q) v[q] = Elem<T>::get(w[q]);
+        } else {
+            each([&](int q) { v[q] = Elem<T>::get(src[q]); });
+        }
+    };
+    const auto put = [&](auto tag, void *to) {
+        constexpr int T = decltype(tag)::value;
+        elem_t<T> *dst = static_cast<elem_t<T> *>(to) + o, w[N];
+#pragma unroll
+        for (int q = 0; q < N; ++q) w[q] = Elem<T>::put(z[q]);
+        if (left >= N) __builtin_memcpy(dst, w, sizeof w);
+        else each([&](int q) { dst[q] = w[q]; });
+    };
+    using D = std::integral_constant<int, DT>;
+    using O = std::integral_constant<int, OT>;
+    using F = std::integral_constant<int, SSMAP_F32>;
+    float v[N] = {};
+    if (p.bias) {
+        if (p.bias_along_m) {
+            const float b = p.bias_f32 ? static_cast<const float *>(p.bias)[m] : Elem<DT>::get(static_cast<const elem_t<DT> *>(p.bias)[m]);
+#pragma unroll
+            for (int q = 0; q < N; ++q) z[q] += b;
+        } else {
+            if (p.bias_f32) get(F{}, p.bias, n, v);
+            else get(D{}, p.bias, n, v);
+#pragma unroll
+            for (int q = 0; q < N; ++q) z[q] += v[q];
+        }
+    }
+    if (p.pre) put(D{}, p.pre);
+    if (p.act) {
+#pragma unroll
+        for (int q = 0; q < N; ++q) z[q] = activate<OT == SSMAP_F32>(z[q], p.act);
+    }
+    if (p.res) {
+        get(O{}, p.res, e * p.res_out + m * p.res_m + n, v);
+#pragma unroll
+        for (int q = 0; q < N; ++q) z[q] += v[q];
+    }
+    put(O{}, p.out);
+}
+
+// BI x BJ results a block, WI x WJ waves.  DIRECT: both sides go straight to LDS (see Side::fetch).
+template <int DT, int OT, bool IK, bool JK, int BI, int BJ, int WI, int WJ, bool DIRECT>
+__global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
+    constexpr int NT = WI * WJ * 64, TI = BI / WI / 16, TJ = BJ / WJ / 16, SIZE = head_dtype_size(DT);
+    using I = Side<DT, IK, BI, NT>;
+    using J = Side<DT, JK, BJ, NT>;
+    constexpr int PITCH = TJ * 16 + 4;                 // floats a row while results are turned: four off, for the banks
+    constexpr int HI = TI > 4 ? TI / 2 : TI;           // rows of 16 turned at once
+    constexpr int STAGE = I::BYTES + J::BYTES, TURN = WI * WJ * HI * 16 * PITCH * 4;
+    __shared__ __attribute__((aligned(1024))) char lds_all[2 * STAGE > TURN ? 2 * STAGE : TURN];
+    const auto stage = [&](int buf) { return lds_all + buf * STAGE; };
+    const int wave = threadIdx.x / 64, wi = wave % WI, wj = wave / WI;
+    const int64_t tiles_m = (p.M + BI - 1) / BI, tiles_n = (p.N + BJ - 1) / BJ, tiles = tiles_m * tiles_n;
+    const int64_t steps = (p.K + I::KB - 1) / I::KB, all_steps = steps * p.sum_batches;
+    const int64_t units = tiles * p.out_batches * p.splits;
+    for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        // Blocks go round the eight XCDs; each takes a run of neighbouring tiles, so that its L2 sees the same
+        // rows again.  Within a run eight tile rows are walked column by column.
+        int64_t id = unit;
+        if (units % 8 == 0) id = (unit % 8) * (units / 8) + unit / 8;
+        const int64_t tile = id % tiles, outer = id / tiles, e = outer % p.out_batches, split = outer / p.out_batches;
+        constexpr int64_t BAND = 8;
+        const int64_t band = tile / (BAND * tiles_n), rows_in = tiles_m - band * BAND < BAND ? tiles_m - band * BAND : BAND;
+        const int64_t in_band = tile % (BAND * tiles_n);
+        const int64_t i0 = (band * BAND + in_band % rows_in) * BI, j0 = in_band / rows_in * BJ;
+        const int rows_i = (int)(p.M - i0 < BI ? p.M - i0 : BI), rows_j = (int)(p.N - j0 < BJ ? p.N - j0 : BJ);
+        const int64_t first = split * p.part_steps, last = first + p.part_steps < all_steps ? first + p.part_steps : all_steps;
+        const int64_t ld_i = (IK ? p.a_m : p.a_k) * SIZE, ld_j = (JK ? p.b_n : p.b_k) * SIZE;
+        const int64_t step_i = (IK ? 1 : p.a_k) * (int64_t)(I::KB * SIZE), step_j = (JK ? 1 : p.b_k) * (int64_t)(I::KB * SIZE);
+        const char *pa = static_cast<const char *>(p.a) + (e * p.a_out + i0 * p.a_m) * SIZE;
+        const char *pb = static_cast<const char *>(p.b) + (e * p.b_out + j0 * p.b_n) * SIZE;
+        int64_t at = first % (steps ? steps : 1);      // stage within its sum batch
+        pa += first / (steps ? steps : 1) * p.a_sum * SIZE + at * step_i;
+        pb += first / (steps ? steps : 1) * p.b_sum * SIZE + at * step_j;
+        const auto advance = [&] {
+            if (++at == steps) {
+                at = 0;
+                pa += p.a_sum * SIZE - (steps - 1) * step_i;
+                pb += p.b_sum * SIZE - (steps - 1) * step_j;
+            } else {
+                pa += step_i;
+                pb += step_j;
+            }
+        };
+        uint32_t off_i[I::PER], off_j[J::PER];
+        i32x4 reg_i[DIRECT ? 1 : I::PER], reg_j[DIRECT ? 1 : J::PER];
+        if constexpr (DIRECT) {
+            I::offsets(off_i, rows_i, I::KB, (uint32_t)ld_i);
+            J::offsets(off_j, rows_j, I::KB, (uint32_t)ld_j);
+        }
+        const auto fetch = [&](int buf) {   // stage `at` into buffer buf (DIRECT) or into registers
+            const int64_t left = p.K - at * I::KB;
+            const int ks = (int)(left < I::KB ? left : I::KB);
+            if constexpr (DIRECT) {
+                const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)stage(buf);
+                if (ks < I::KB) {
+                    uint32_t tail_i[I::PER], tail_j[J::PER];
+                    I::offsets(tail_i, rows_i, ks, (uint32_t)ld_i);
+                    J::offsets(tail_j, rows_j, ks, (uint32_t)ld_j);
+                    I::fetch(pa, tail_i, base);
+                    J::fetch(pb, tail_j, base + I::BYTES);
+                } else {
+                    I::fetch(pa, off_i, base);
+                    J::fetch(pb, off_j, base + I::BYTES);
+                }
+            } else {
+                I::load(reg_i, pa, rows_i, ks, ld_i);
+                J::load(reg_j, pb, rows_j, ks, ld_j);
+            }
+            advance();
+        };
+        const auto keep = [&](int buf) {
+            if constexpr (!DIRECT) {
+                I::store(reg_i, stage(buf));
+                J::store(reg_j, stage(buf) + I::BYTES);
+            }
+        };
+        f32x4 acc[TI][TJ] = {};
+        if (first < last) {
+            fetch(0);
+            keep(0);
+        }
+        for (int64_t t = first; t < last; ++t) {
+            const int buf = (int)((t - first) & 1);
+            // this wave's part of the stage has landed; behind the barrier everybody's has, and nobody reads
+            // the other buffer any more
+            if constexpr (DIRECT) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            const bool more = t + 1 < last;
+            if (more) fetch(buf ^ 1);
+            const char *li = stage(buf), *lj = li + I::BYTES;
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                i32x4 fi[TI], fj[TJ];
+#pragma unroll
+                for (int i = 0; i < TI; ++i) fi[i] = I::read(li, (wi * TI + i) * 16, kk);
+#pragma unroll
+                for (int j = 0; j < TJ; ++j) fj[j] = J::read(lj, (wj * TJ + j) * 16, kk);
+#pragma unroll
+                for (int i = 0; i < TI; ++i)
+#pragma unroll
+                    for (int j = 0; j < TJ; ++j) acc[i][j] = mma_chunk<DT>(fj[j], fi[i], acc[i][j]);
+            }
+            if (more) keep(buf ^ 1);
+        }
+        __syncthreads();   // nobody reads the stages any more
+        // Each wave turns its own results round in LDS, HI rows of 16 at a time: out of the registers with four
+        // neighbouring n a lane, back with eight, so that the epilogue is one loop over whole rows.
+        const int lane = threadIdx.x % 64, q = lane % 16, g = lane / 16;
+        float *turn = reinterpret_cast<float *>(lds_all + wave * (HI * 16 * PITCH * 4));
+#pragma unroll
+        for (int h = 0; h < TI / HI; ++h) {
+#pragma unroll
+            for (int i = 0; i < HI; ++i)
+#pragma unroll
+                for (int j = 0; j < TJ; ++j) *reinterpret_cast<f32x4 *>(turn + (i * 16 + q) * PITCH + j * 16 + g * 4) = acc[h * HI + i][j];
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");   // the wave's own writes, in order
+            __builtin_amdgcn_wave_barrier();
+            constexpr int LINE = TJ * 16 / 8;   // lanes a row
+#pragma unroll 1
+            for (int u = lane; u < HI * 16 * LINE; u += 64) {
+                const int row = u / LINE, col = u % LINE * 8;
+                const int64_t m = i0 + (wi * TI + h * HI) * 16 + row, n = j0 + wj * TJ * 16 + col;
+                const int left = (int)(p.N - n < 8 ? p.N - n : 8);
+                if (m >= p.M || left <= 0) continue;
+                const int64_t o = (e * p.M + m) * p.N + n;
+                float z[8];
+                __builtin_memcpy(z, turn + row * PITCH + col, 32);
+                if (p.splits > 1) {
+                    float *part = p.parts + split * p.out_batches * p.M * p.N + o;
+                    if (left == 8) __builtin_memcpy(part, z, 32);
+                    else {
+#pragma unroll
+                        for (int s = 0; s < 8; ++s)
+                            if (s < left) part[s] = z[s];
+                    }
+                } else {
+                    finish<DT, OT, 8>(p, o, e, m, n, left, z);
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+        __syncthreads();   // the next tile's first stage overwrites the buffers
+    }
+}
+
+// Joins the partial results of a split sum, in the splits' order, and finishes them.
+template <int DT, int OT>
+__global__ __launch_bounds__(256) void k_join_parts(Product p) {
+    const int64_t row = (p.N + 3) / 4, units = p.out_batches * p.M * row;
+    for (int64_t u = blockIdx.x * 256ll + threadIdx.x; u < units; u += gridDim.x * 256ll) {
+        const int64_t em = u / row, e = em / p.M, m = em % p.M, n = u % row * 4, o = em * p.N + n;
+        const int left = (int)(p.N - n < 4 ? p.N - n : 4);
+        float z[4] = {};
+        for (int s = 0; s < p.splits; ++s) {
+            const float *part = p.parts + s * p.out_batches * p.M * p.N + o;
+            float v[4] = {};
+            if (left == 4) __builtin_memcpy(v, part, 16);
+            else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (q < left) v[q] = part[q];
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) z[q] += v[q];
+        }
+        finish<DT, OT, 4>(p, o, e, m, n, left, z);
+    }
+}
+
+// Whether a side can go straight to LDS: lines at multiples of 16 bytes, no partial chunk, 32-bit offsets
+// within a tile.
+inline bool direct_side(const void *p, int64_t line, int64_t out, int64_t sum, int64_t dense, int size) {
+    const int64_t e = 16 / size;
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && line % e == 0 && out % e == 0 && sum % e == 0 && dense % e == 0 &&
+           line >= 0 && line < (int64_t)1 << 21;
+}
+
+template <int DT, int OT, bool IK, bool JK>
+void launch_tiles(Product p, hipStream_t st) {
+    const int size = head_dtype_size(DT);
+    const bool direct = direct_side(p.a, IK ? p.a_m : p.a_k, p.a_out, p.a_sum, IK ? p.K : p.M, size) &&
+                        direct_side(p.b, JK ? p.b_n : p.b_k, p.b_out, p.b_sum, JK ? p.K : p.N, size);
+    p.splits = 1;
+    p.part_steps = (p.K * size + 127) / 128 * p.sum_batches;
+    const auto tiles = [&](int bi, int bj) { return (p.M + bi - 1) / bi * ((p.N + bj - 1) / bj) * p.out_batches; };
+    const auto go = [&](auto bi, auto bj, auto wi, auto wj, auto d) {
+        k_tiles<DT, OT, IK, JK, bi.value, bj.value, wi.value, wj.value, d.value>
+            <<<blocks(tiles(bi.value, bj.value) * p.splits), wi.value * wj.value * 64, 0, st>>>(p);
+    };
+    using std::integral_constant;
+    const integral_constant<int, 2> two{};
+    const integral_constant<int, 4> four{};
+    const integral_constant<int, 128> small{};
+    const integral_constant<int, 256> big{};
+    if (p.M * p.N * p.out_batches == 0) return;
+    if (!direct) go(small, small, two, two, std::false_type{});
+    // two rounds of the large tile and more: 1177 against 1084 TFLOP/s at 8192^3 bf16; at one round (4096^3) they are equal
+    else if (DT != SSMAP_F32 && tiles(256, 256) >= 512) go(big, big, two, four, std::true_type{});
+    else go(small, small, two, two, std::true_type{});
+}
+
+template <int DT, int OT>
+void launch_product(const Product &p, hipStream_t st) {
+    if (p.a_k == 1 && p.b_k == 1) launch_tiles<DT, OT, true, true>(p, st);
+    else if constexpr (DT == OT) {
+        if (p.a_k == 1) launch_tiles<DT, OT, true, false>(p, st);
+        else launch_tiles<DT, OT, false, false>(p, st);
+    }
+}
+
+}  // namespace ssmap

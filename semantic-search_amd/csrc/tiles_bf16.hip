@@ -1,0 +1,12 @@
+// The matrix products of bfloat16 operands.
+#include <math.h>
+#include <stdlib.h>
+
+#include "tiles.h"
+
+namespace ssmap {
+
+template void launch_product<SSMAP_BF16, SSMAP_BF16>(const Product &, hipStream_t);
+template void launch_product<SSMAP_BF16, SSMAP_F32>(const Product &, hipStream_t);
+
+}  // namespace ssmap

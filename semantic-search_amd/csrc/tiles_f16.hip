@@ -1,0 +1,12 @@
+// The matrix products of float16 operands.
+#include <math.h>
+#include <stdlib.h>
+
+#include "tiles.h"
+
+namespace ssmap {
+
+template void launch_product<SSMAP_F16, SSMAP_F16>(const Product &, hipStream_t);
+template void launch_product<SSMAP_F16, SSMAP_F32>(const Product &, hipStream_t);
+
+}  // namespace ssmap

@@ -1,0 +1,11 @@
+// The matrix products of float32 operands.
+#include <math.h>
+#include <stdlib.h>
+
+#include "tiles.h"
+
+namespace ssmap {
+
+template void launch_product<SSMAP_F32, SSMAP_F32>(const Product &, hipStream_t);
+
+}  // namespace ssmap
