@@ -6,65 +6,133 @@
 // a position, so that the dense axis of the planes is the dense axis of the tiles.
 #include <math.h>
 
-#include "heads.h"
 #include "products.h"
-#include "tiles.h"
 
 using namespace ssmap;
 
 namespace {
 
-__device__ __forceinline__ float slope(float z, int act) {
-    if (act == SSMAP_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
-    if (act == SSMAP_ACT_GELU)
-        return 0.5f * erfcf(-0.70710678118654752f * z) + z * 0.39894228040143268f * expf(-0.5f * z * z);
-    if (act == SSMAP_ACT_GELU_TANH) {
-        const float u = 0.79788456080286536f * (z + 0.044715f * z * z * z);
-        const float q = 1.0f / (1.0f + expf(-2.0f * u));     // (1 + tanh u) / 2; its slope in u is 2 q (1 - q)
-        const float du = 0.79788456080286536f * (1.0f + 3.0f * 0.044715f * z * z);
-        return q + (1.0f - q > 0.0f && q > 0.0f ? z * 2.0f * q * (1.0f - q) * du : 0.0f);
-    }
-    if (act == SSMAP_ACT_SILU) {
-        const float q = 1.0f / (1.0f + expf(-z));
-        return q + (q > 0.0f && q < 1.0f ? z * q * (1.0f - q) : 0.0f);
-    }
-    return 1.0f;
+// Whether a side can go straight to LDS: lines at multiples of 16 bytes, no partial chunk, 32-bit offsets
+// within a tile.
+inline bool direct_side(const void *p, int64_t line, int64_t out, int64_t sum, int64_t dense, int size) {
+    const int64_t e = 16 / size;
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && line % e == 0 && out % e == 0 && sum % e == 0 && dense % e == 0 &&
+           line >= 0 && line < (int64_t)1 << 21;
 }
 
-// dz = g act'(pre) in the products' type, dense.  out: [batch][P][Q], g strided by (batch, P).
-template <int DT, int OT>
-__global__ __launch_bounds__(256) void k_dz(int64_t batch, int64_t P, int64_t Q, const elem_t<OT> *g, int64_t g_batch, int64_t g_p,
-                                            const elem_t<DT> *pre, int act, elem_t<DT> *dz) {
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < batch * P * Q; i += gridDim.x * 256ll) {
-        const int64_t q = i % Q, pp = i / Q % P, b = i / Q / P;
-        float v = Elem<OT>::get(g[b * g_batch + pp * g_p + q]);
-        if (pre) v *= slope(Elem<DT>::get(pre[i]), act);
-        dz[i] = Elem<DT>::put(v);
-    }
-}
+// dz = g act'(pre) in the products' type, dense, and the sums of its positions for the bias's gradient, in one
+// pass over g.  [batch][P][Q], Q dense: rows have the outputs in Q, planes in P.
+constexpr int kDzRows = 128;       // rows: positions a block sums; 8 threads down, 32 packs of 8 outputs across
+constexpr int kDzPlane = 16384;    // planes: positions a block sums
 
-// g_bias: one block per output sums its dz over the positions, each thread a fixed share, joined in a fixed order.
 template <int DT, int OT>
-__global__ __launch_bounds__(256) void k_bias_grad(int64_t batch, int64_t rows, int64_t outer, const elem_t<OT> *g, int64_t g_batch,
-                                                   int64_t g_row, int64_t g_out, const elem_t<DT> *pre, int64_t pre_row, int64_t pre_out,
-                                                   int act, elem_t<DT> *out) {
-    __shared__ float part[256];
-    for (int64_t n = blockIdx.x; n < outer; n += gridDim.x) {
-        float s = 0.0f;
-        for (int64_t i = threadIdx.x; i < batch * rows; i += 256) {
-            const int64_t b = i / rows, r = i % rows;
-            float v = Elem<OT>::get(g[b * g_batch + r * g_row + n * g_out]);
-            if (pre) v *= slope(Elem<DT>::get(pre[b * rows * outer + r * pre_row + n * pre_out]), act);
-            s += v;
+__device__ __forceinline__ void dz_pack(const elem_t<OT> *g, const elem_t<DT> *pre, elem_t<DT> *dz, int left, int act, float (&sum)[8]) {
+    float v[8] = {};
+    if (left >= 8) {
+        elem_t<OT> w[8];
+        __builtin_memcpy(w, g, sizeof w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = Elem<OT>::get(w[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < left) v[e] = Elem<OT>::get(g[e]);
+    }
+    if (pre) {
+        float z[8] = {};
+        if (left >= 8) {
+            elem_t<DT> w[8];
+            __builtin_memcpy(w, pre, sizeof w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z[e] = Elem<DT>::get(w[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < left) z[e] = Elem<DT>::get(pre[e]);
         }
-        part[threadIdx.x] = s;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= slope<DT == SSMAP_F32>(z[e], act);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum[e] += v[e];
+    if (dz) {
+        elem_t<DT> w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = Elem<DT>::put(v[e]);
+        if (left >= 8) {
+            __builtin_memcpy(dz, w, sizeof w);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (e < left) dz[e] = w[e];
+        }
+    }
+}
+
+// sums[batch * row chunks][outer]
+template <int DT, int OT>
+__global__ __launch_bounds__(256) void k_dz_rows(int64_t batch, int64_t rows, int64_t outer, const elem_t<OT> *g, int64_t g_batch, int64_t g_row,
+                                                 const elem_t<DT> *pre, int act, elem_t<DT> *dz, float *sums) {
+    __shared__ float part[8][256];
+    const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+    const int64_t strips = (outer + 255) / 256, chunks = (rows + kDzRows - 1) / kDzRows;
+    for (int64_t unit = blockIdx.x; unit < strips * chunks * batch; unit += gridDim.x) {
+        const int64_t n = unit % strips * 256 + tx * 8, bc = unit / strips, b = bc / chunks, r0 = bc % chunks * kDzRows;
+        const int left = (int)(outer - n < 8 ? outer - n : 8);
+        float sum[8] = {};
+        if (left > 0)
+            for (int64_t r = r0 + ty; r < r0 + kDzRows && r < rows; r += 8) {
+                const int64_t o = (b * rows + r) * outer + n;
+                dz_pack<DT, OT>(g + b * g_batch + r * g_row + n, pre ? pre + o : nullptr, dz ? dz + o : nullptr, left, act, sum);
+            }
+        if (!sums) continue;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) part[ty][tx * 8 + e] = sum[e];
+        __syncthreads();
+        const int64_t out = unit % strips * 256 + threadIdx.x;
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s += part[k][threadIdx.x];
+        if (out < outer) sums[bc * outer + out] = s;
+    }
+}
+
+// sums[batch * chunks][outer]
+template <int DT, int OT>
+__global__ __launch_bounds__(256) void k_dz_planes(int64_t batch, int64_t rows, int64_t outer, const elem_t<OT> *g, int64_t g_batch, int64_t g_plane,
+                                                   const elem_t<DT> *pre, int act, elem_t<DT> *dz, float *sums) {
+    __shared__ float part[256];
+    const int64_t chunks = (rows + kDzPlane - 1) / kDzPlane;
+    for (int64_t unit = blockIdx.x; unit < chunks * outer * batch; unit += gridDim.x) {
+        const int64_t c = unit % chunks, bn = unit / chunks, b = bn / outer, n = bn % outer;
+        float sum[8] = {};
+        const int64_t end = (c + 1) * kDzPlane < rows ? (c + 1) * kDzPlane : rows;
+        for (int64_t r = c * kDzPlane + threadIdx.x * 8; r < end; r += 2048) {
+            const int64_t o = bn * rows + r;
+            dz_pack<DT, OT>(g + b * g_batch + n * g_plane + r, pre ? pre + o : nullptr, dz ? dz + o : nullptr, (int)(end - r < 8 ? end - r : 8), act, sum);
+        }
+        if (!sums) continue;
+        part[threadIdx.x] = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
         __syncthreads();
         for (int d = 128; d; d >>= 1) {
             if (threadIdx.x < d) part[threadIdx.x] += part[threadIdx.x + d];
             __syncthreads();
         }
-        if (!threadIdx.x) out[n] = Elem<DT>::put(part[0]);
+        if (!threadIdx.x) sums[(b * chunks + c) * outer + n] = part[0];
         __syncthreads();
+    }
+}
+
+// g_bias from the chunks' sums: a wave takes 64 chunks of one output at a time.
+template <int DT>
+__global__ __launch_bounds__(256) void k_bias_grad(int64_t chunks, int64_t outer, const float *sums, elem_t<DT> *out) {
+    for (int64_t n = blockIdx.x * 4ll + threadIdx.x / 64; n < outer; n += gridDim.x * 4ll) {
+        float s = 0.0f;
+        for (int64_t c = threadIdx.x % 64; c < chunks; c += 64) s += sums[c * outer + n];
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
+        if (threadIdx.x % 64 == 0) out[n] = Elem<DT>::put(s);
     }
 }
 
@@ -103,20 +171,18 @@ int check_grad(const ssmap_linear_grad_args *a) {
     return check(a, a->grad_dtype);
 }
 
+// The workspace of ssmap_linear_grad: dz, the bias's sums, the partial results of the products (one after
+// the other, so they share a place).
+struct GradPlan {
+    bool planes, copies;               // copies: dz differs from g
+    int64_t chunks;                    // sums a block leaves for each output
+    Product x, w;
+    int64_t dz_bytes, sum_bytes, part_bytes;
+};
+
 inline int64_t aligned(int64_t bytes) { return (bytes + 255) & ~(int64_t)255; }
 
-}  // namespace
-
-extern "C" {
-
-int64_t ssmap_linear_workspace(const ssmap_linear_args *a) { return check_linear(a) == SSMAP_OK ? 0 : -1; }
-
-int ssmap_linear(const ssmap_linear_args *a, void *stream) {
-    if (int rc = check_linear(a)) return rc;
-    const int64_t positions = a->batch * a->rows;
-    if (positions == 0 || a->outer == 0) return SSMAP_OK;
-    if (!a->y || (a->inner && (!a->x || !a->w))) return head_error(SSMAP_ERR_INVALID_ARG, "null argument");
-    if (a->workspace_bytes < ssmap_linear_workspace(a)) return head_error(SSMAP_ERR_INVALID_ARG, "the workspace is smaller than ssmap_linear_workspace says");
+Product forward_product(const ssmap_linear_args *a) {
     const bool planes = a->layout == SSMAP_PLANES;
     Product p{};
     p.K = a->inner; p.out_batches = a->batch; p.sum_batches = 1;
@@ -132,13 +198,64 @@ int ssmap_linear(const ssmap_linear_args *a, void *stream) {
         p.a = a->x; p.a_m = a->x_row_stride; p.a_k = 1; p.a_out = a->x_batch_stride;
         p.b = a->w; p.b_n = a->w_row_stride; p.b_k = 1;
     }
+    return p;
+}
+
+GradPlan plan_grad(const ssmap_linear_grad_args *a) {
+    GradPlan q{};
+    q.planes = a->layout == SSMAP_PLANES;
+    q.copies = a->activation != SSMAP_ACT_NONE || a->grad_dtype != a->dtype;
+    const int64_t chunk = q.planes ? kDzPlane : kDzRows;
+    q.chunks = a->batch * ((a->rows + chunk - 1) / chunk);
+    q.dz_bytes = q.copies && (a->g_x || a->g_w) ? aligned(a->batch * a->rows * a->outer * head_dtype_size(a->dtype)) : 0;
+    q.sum_bytes = a->g_bias ? aligned(q.chunks * a->outer * 4) : 0;
+    // dz: [position][output] or [output][position] of a batch
+    const void *dz = q.copies ? a->workspace : a->g;
+    const int64_t line = q.copies ? (q.planes ? a->rows : a->outer) : a->g_inner_stride, batch = q.copies ? a->rows * a->outer : a->g_batch_stride;
+    const int64_t to_row = q.planes ? 1 : line, to_out = q.planes ? line : 1;
+    Product &x = q.x;
+    x.M = a->rows; x.N = a->inner; x.K = a->outer; x.out_batches = a->batch; x.sum_batches = 1;
+    x.a = dz; x.a_out = batch; x.a_m = to_row; x.a_k = to_out;
+    x.b = a->w; x.b_n = 1; x.b_k = a->w_row_stride;
+    x.out = a->g_x;
+    Product &w = q.w;
+    w.M = a->outer; w.N = a->inner; w.K = a->rows; w.out_batches = 1; w.sum_batches = a->batch;
+    w.a = dz; w.a_sum = batch; w.a_m = to_out; w.a_k = to_row;
+    w.b = a->x; w.b_sum = a->x_batch_stride; w.b_n = 1; w.b_k = a->x_row_stride;
+    w.out = a->g_w;
+    const int64_t need_x = a->g_x ? plan_product(x, a->dtype) : 0, need_w = a->g_w ? plan_product(w, a->dtype) : 0;
+    q.part_bytes = aligned(need_x > need_w ? need_x : need_w);
+    return q;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t ssmap_linear_workspace(const ssmap_linear_args *a) {
+    if (check_linear(a) != SSMAP_OK) return -1;
+    Product p = forward_product(a);
+    return plan_product(p, a->dtype);
+}
+
+int ssmap_linear(const ssmap_linear_args *a, void *stream) {
+    if (int rc = check_linear(a)) return rc;
+    const int64_t positions = a->batch * a->rows;
+    if (positions == 0 || a->outer == 0) return SSMAP_OK;
+    if (!a->y || (a->inner && (!a->x || !a->w))) return head_error(SSMAP_ERR_INVALID_ARG, "null argument");
+    Product p = forward_product(a);
+    const int64_t need = plan_product(p, a->dtype);
+    if (a->workspace_bytes < need || (need && (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 16)))
+        return head_error(SSMAP_ERR_INVALID_ARG, "the workspace is not at a multiple of 16 or smaller than ssmap_linear_workspace says");
+    p.parts = static_cast<float *>(a->workspace);
     with_types(a->dtype, a->out_dtype, [&](auto dt, auto ot) { launch_product<dt.value, ot.value>(p, static_cast<hipStream_t>(stream)); });
     return head_launch_error(hipGetLastError());
 }
 
 int64_t ssmap_linear_grad_workspace(const ssmap_linear_grad_args *a) {
     if (check_grad(a) != SSMAP_OK) return -1;
-    return aligned(a->batch * a->rows * a->outer * head_dtype_size(a->dtype));
+    const GradPlan q = plan_grad(a);
+    return q.dz_bytes + q.sum_bytes + q.part_bytes;
 }
 
 int ssmap_linear_grad(const ssmap_linear_grad_args *a, void *stream) {
@@ -148,42 +265,69 @@ int ssmap_linear_grad(const ssmap_linear_grad_args *a, void *stream) {
     if (a->activation != SSMAP_ACT_NONE && positions && a->outer && !a->pre) return head_error(SSMAP_ERR_INVALID_ARG, "an activation's gradient needs pre");
     if ((a->g_x && positions && a->inner && a->outer && !a->w) || (a->g_w && a->outer && a->inner && positions && !a->x))
         return head_error(SSMAP_ERR_INVALID_ARG, "null argument");
-    const int64_t need = ssmap_linear_grad_workspace(a);
-    if (a->workspace_bytes < need || (need && !a->workspace))
-        return head_error(SSMAP_ERR_INVALID_ARG, "the workspace is smaller than ssmap_linear_grad_workspace says");
-    const bool planes = a->layout == SSMAP_PLANES;
+    GradPlan q = plan_grad(a);
+    const int64_t need = q.dz_bytes + q.sum_bytes + q.part_bytes;
+    if (a->workspace_bytes < need || (need && (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 16)))
+        return head_error(SSMAP_ERR_INVALID_ARG, "the workspace is not at a multiple of 16 or smaller than ssmap_linear_grad_workspace says");
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const void *pre = a->activation == SSMAP_ACT_NONE ? nullptr : a->pre;
+    char *ws = static_cast<char *>(a->workspace);
+    float *sums = q.sum_bytes ? reinterpret_cast<float *>(ws + q.dz_bytes) : nullptr;
+    q.x.parts = q.w.parts = reinterpret_cast<float *>(ws + q.dz_bytes + q.sum_bytes);
     with_types(a->dtype, a->grad_dtype, [&](auto dt, auto ot) {
         constexpr int DT = dt.value, OT = ot.value;
-        const int64_t P = planes ? a->outer : a->rows, Q = planes ? a->rows : a->outer;
         const auto *g = static_cast<const elem_t<OT> *>(a->g);
-        auto *dz = static_cast<elem_t<DT> *>(a->workspace);
-        const auto *z = static_cast<const elem_t<DT> *>(pre);
-        if (positions * a->outer)
-            k_dz<DT, OT><<<blocks((positions * a->outer + 255) / 256), 256, 0, st>>>(a->batch, P, Q, g, a->g_batch_stride, a->g_inner_stride, z, a->activation, dz);
-        if (a->g_bias && a->outer)
-            k_bias_grad<DT, OT><<<blocks(a->outer), 256, 0, st>>>(a->batch, a->rows, a->outer, g, a->g_batch_stride, planes ? 1 : a->g_inner_stride,
-                                                                  planes ? a->g_inner_stride : 1, z, planes ? 1 : a->outer, planes ? a->rows : 1,
-                                                                  a->activation, static_cast<elem_t<DT> *>(a->g_bias));
-        if (a->g_x) {
-            Product p{};
-            p.M = a->rows; p.N = a->inner; p.K = a->outer; p.out_batches = a->batch; p.sum_batches = 1;
-            p.a = dz; p.a_out = a->rows * a->outer; p.a_m = planes ? 1 : a->outer; p.a_k = planes ? a->rows : 1;
-            p.b = a->w; p.b_n = 1; p.b_k = a->w_row_stride;
-            p.out = a->g_x;
-            launch_product<DT, DT>(p, st);
+        const auto *pre = a->activation == SSMAP_ACT_NONE ? nullptr : static_cast<const elem_t<DT> *>(a->pre);
+        auto *dz = q.dz_bytes ? reinterpret_cast<elem_t<DT> *>(ws) : nullptr;
+        if (positions * a->outer && (dz || sums)) {
+            if (q.planes)
+                k_dz_planes<DT, OT><<<blocks(q.chunks * a->outer), 256, 0, st>>>(a->batch, a->rows, a->outer, g, a->g_batch_stride, a->g_inner_stride, pre, a->activation, dz, sums);
+            else
+                k_dz_rows<DT, OT><<<blocks(q.chunks * ((a->outer + 255) / 256)), 256, 0, st>>>(a->batch, a->rows, a->outer, g, a->g_batch_stride, a->g_inner_stride, pre, a->activation, dz, sums);
         }
-        if (a->g_w) {
-            Product p{};
-            p.M = a->outer; p.N = a->inner; p.K = a->rows; p.out_batches = 1; p.sum_batches = a->batch;
-            p.a = dz; p.a_sum = a->rows * a->outer; p.a_m = planes ? a->rows : 1; p.a_k = planes ? 1 : a->outer;
-            p.b = a->x; p.b_sum = a->x_batch_stride; p.b_n = 1; p.b_k = a->x_row_stride;
-            p.out = a->g_w;
-            launch_product<DT, DT>(p, st);
-        }
+        if (a->g_bias && a->outer) k_bias_grad<DT><<<blocks((a->outer + 3) / 4), 256, 0, st>>>(q.chunks, a->outer, sums, static_cast<elem_t<DT> *>(a->g_bias));
+        if (a->g_x) launch_product<DT, DT>(q.x, st);
+        if (a->g_w) launch_product<DT, DT>(q.w, st);
     });
     return head_launch_error(hipGetLastError());
 }
 
 }  // extern "C"
+
+int64_t ssmap::plan_product(Product &p, int dtype) {
+    const int size = head_dtype_size(dtype);
+    const bool ik = p.a_k == 1, jk = p.b_k == 1;
+    p.splits = 1;
+    const int64_t steps = (p.K * size + 127) / 128 * p.sum_batches;
+    p.part_steps = steps;
+    const bool direct = direct_side(p.a, ik ? p.a_m : p.a_k, p.a_out, p.a_sum, ik ? p.K : p.M, size) &&
+                        direct_side(p.b, jk ? p.b_n : p.b_k, p.b_out, p.b_sum, jk ? p.K : p.N, size);
+    const auto tiles = [&](int bi, int bj) { return (p.M + bi - 1) / bi * ((p.N + bj - 1) / bj) * p.out_batches; };
+    if (p.M <= kFewMost && ik && jk && p.sum_batches == 1 && (p.K * size >= 2048 || tiles(64, 256) < 512)) {
+        p.shape = kFewRows;
+        return 0;
+    }
+    int64_t units = tiles(128, 128), full = 512;   // tiles, and how many are resident at once
+    if (!direct) {
+        p.shape = kTileMidAny;
+    } else if (p.M <= 64) {
+        p.shape = kTileLow;
+        units = tiles(64, 256);
+    } else if (p.N <= 64) {
+        p.shape = kTileTall;
+        units = tiles(256, 64);
+    } else if (dtype != SSMAP_F32 && tiles(256, 256) >= 512) {
+        // two rounds of the large tile and more: 1177 against 1084 TFLOP/s at 8192^3 bf16; at one round (4096^3)
+        // they are equal
+        p.shape = kTileBig;
+        units = tiles(256, 256), full = 256;
+    } else {
+        p.shape = kTileMid;
+    }
+    // Fewer than half of the tiles that fit at once: the sum is split, in parts of eight stages at least
+    if (units && units * 2 <= full && steps >= 16) {
+        const int64_t most = steps / 8, want = full / units < most ? full / units : most;
+        p.part_steps = (steps + want - 1) / want;
+        p.splits = (int)((steps + p.part_steps - 1) / p.part_steps);
+    }
+    return p.splits > 1 ? aligned(p.splits * p.out_batches * p.M * p.N * 4) : 0;
+}

@@ -1,6 +1,8 @@
 // A product of linear.hip and the launcher of its kernels, which are compiled one operand type a file.
 #pragma once
 
+#include <math.h>
+
 #include "heads.h"
 
 namespace ssmap {
@@ -20,13 +22,66 @@ struct Product {
     // the sum is split into `splits` parts of `part_steps` stages; more than one: float32 partial results go to
     // parts[split][out_batches][M][N] and are joined afterwards
     int64_t part_steps;
-    int32_t splits, pad2;
+    int32_t splits, shape;                  // shape: see plan_product
     float *parts;
 };
 
+// Tile shapes (m x n).
+enum Shape { kTileBig = 0, kTileMid = 1, kTileLow = 2, kTileTall = 3, kTileMidAny = 4, kFewRows = 5 };
+constexpr int kFewMost = 32;                // rows kFewRows takes at most
+
 inline unsigned blocks(int64_t n) { return (unsigned)(n < 1 ? 1 : n < (1 << 20) ? n : (1 << 20)); }
 
-// Enqueues a product of operands of type DT with results of type OT (DT or SSMAP_F32).
+// Chooses p.shape, p.splits and p.part_steps by sizes, strides and alignment; returns the bytes that p.parts needs.
+int64_t plan_product(Product &p, int dtype);
+// FINE: for results in float32.  Results of 16 bits take erfc from Abramowitz and Stegun's formula 7.1.26,
+// whose error of 1.5e-7 is far below their rounding.
+template <bool FINE>
+__device__ __forceinline__ float half_erfc(float x) {   // erfc(x) / 2
+    if constexpr (FINE) return 0.5f * erfcf(x);
+    const float a = fabsf(x), t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * a);
+    const float y = t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f))));
+    const float v = y * __builtin_amdgcn_exp2f(-1.44269504088896341f * a * a);
+    return x < 0.0f ? 1.0f - v : v;
+}
+template <bool FINE>
+__device__ __forceinline__ float logistic(float x) {    // 1 / (1 + exp(-x))
+    if constexpr (FINE) return 1.0f / (1.0f + expf(-x));
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * x));
+}
+template <bool FINE>
+__device__ __forceinline__ float activate(float z, int act) {
+    if (act == SSMAP_ACT_RELU) return z < 0.0f ? 0.0f : z;
+    if (act == SSMAP_ACT_GELU) return z * half_erfc<FINE>(-0.70710678118654752f * z);
+    if (act == SSMAP_ACT_GELU_TANH) {
+        // (1 + tanh u) / 2 = 1 / (1 + exp(-2u))
+        return z * logistic<FINE>(1.5957691216057308f * (z + 0.044715f * z * z * z));
+    }
+    if (act == SSMAP_ACT_SILU) return z * logistic<FINE>(z);
+    return z;
+}
+
+template <bool FINE>
+__device__ __forceinline__ float slope(float z, int act) {
+    if (act == SSMAP_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+    if (act == SSMAP_ACT_GELU) {
+        const float bell = FINE ? expf(-0.5f * z * z) : __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
+        return half_erfc<FINE>(-0.70710678118654752f * z) + z * 0.39894228040143268f * bell;
+    }
+    if (act == SSMAP_ACT_GELU_TANH) {
+        // q = (1 + tanh u) / 2; its slope in u is 2 q (1 - q), which is 0 where z may be infinite
+        const float q = logistic<FINE>(1.5957691216057308f * (z + 0.044715f * z * z * z));
+        const float du = 0.79788456080286536f * (1.0f + 3.0f * 0.044715f * z * z);
+        return q + (q > 0.0f && q < 1.0f ? z * 2.0f * q * (1.0f - q) * du : 0.0f);
+    }
+    if (act == SSMAP_ACT_SILU) {
+        const float q = logistic<FINE>(z);
+        return q + (q > 0.0f && q < 1.0f ? z * q * (1.0f - q) : 0.0f);
+    }
+    return 1.0f;
+}
+
+// Enqueues a planned product of operands of type DT with results of type OT (DT or SSMAP_F32).
 template <int DT, int OT>
 void launch_product(const Product &p, hipStream_t st);
 

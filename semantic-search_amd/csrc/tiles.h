@@ -143,33 +143,6 @@ struct Side {
     }
 };
 
-// FINE: for results in float32.  Results of 16 bits take erfc from Abramowitz and Stegun's formula 7.1.26,
-// whose error of 1.5e-7 is far below their rounding.
-template <bool FINE>
-__device__ __forceinline__ float half_erfc(float x) {   // erfc(x) / 2
-    if constexpr (FINE) return 0.5f * erfcf(x);
-    const float a = fabsf(x), t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * a);
-    const float y = t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f))));
-    const float v = y * __builtin_amdgcn_exp2f(-1.44269504088896341f * a * a);
-    return x < 0.0f ? 1.0f - v : v;
-}
-template <bool FINE>
-__device__ __forceinline__ float logistic(float x) {    // 1 / (1 + exp(-x))
-    if constexpr (FINE) return 1.0f / (1.0f + expf(-x));
-    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * x));
-}
-template <bool FINE>
-__device__ __forceinline__ float activate(float z, int act) {
-    if (act == SSMAP_ACT_RELU) return z < 0.0f ? 0.0f : z;
-    if (act == SSMAP_ACT_GELU) return z * half_erfc<FINE>(-0.70710678118654752f * z);
-    if (act == SSMAP_ACT_GELU_TANH) {
-        // (1 + tanh u) / 2 = 1 / (1 + exp(-2u))
-        return z * logistic<FINE>(1.5957691216057308f * (z + 0.044715f * z * z * z));
-    }
-    if (act == SSMAP_ACT_SILU) return z * logistic<FINE>(z);
-    return z;
-}
-
 // N results next to each other (n, n + 1, ...), of which `left` exist.  `o` is the first one's place in the
 // dense output.
 template <int DT, int OT, int N>
@@ -374,68 +347,158 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
     }
 }
 
-// Joins the partial results of a split sum, in the splits' order, and finishes them.
-template <int DT, int OT>
+// Joins the partial results of a split sum and finishes them: 256 / LANES quads of results a block, LANES
+// threads a quad, each over its share of the splits; joined in a fixed order.
+template <int DT, int OT, int LANES>
 __global__ __launch_bounds__(256) void k_join_parts(Product p) {
+    constexpr int QUADS = 256 / LANES;
+    __shared__ f32x4 sums[LANES][QUADS];
     const int64_t row = (p.N + 3) / 4, units = p.out_batches * p.M * row;
-    for (int64_t u = blockIdx.x * 256ll + threadIdx.x; u < units; u += gridDim.x * 256ll) {
+    const int quad = threadIdx.x % QUADS, part = threadIdx.x / QUADS;
+    for (int64_t u0 = blockIdx.x * (int64_t)QUADS; u0 < units; u0 += gridDim.x * (int64_t)QUADS) {
+        const int64_t u = u0 + quad < units ? u0 + quad : units - 1;
         const int64_t em = u / row, e = em / p.M, m = em % p.M, n = u % row * 4, o = em * p.N + n;
         const int left = (int)(p.N - n < 4 ? p.N - n : 4);
         float z[4] = {};
-        for (int s = 0; s < p.splits; ++s) {
-            const float *part = p.parts + s * p.out_batches * p.M * p.N + o;
+#pragma unroll 4
+        for (int s = part; s < p.splits; s += LANES) {
+            const float *from = p.parts + s * p.out_batches * p.M * p.N + o;
             float v[4] = {};
-            if (left == 4) __builtin_memcpy(v, part, 16);
+            if (left == 4) __builtin_memcpy(v, from, 16);
             else {
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
-                    if (q < left) v[q] = part[q];
+                    if (q < left) v[q] = from[q];
             }
 #pragma unroll
             for (int q = 0; q < 4; ++q) z[q] += v[q];
         }
-        finish<DT, OT, 4>(p, o, e, m, n, left, z);
+        if constexpr (LANES > 1) {
+            __syncthreads();
+            sums[part][quad] = f32x4{z[0], z[1], z[2], z[3]};
+            __syncthreads();
+            if (part == 0)
+#pragma unroll
+                for (int k = 1; k < LANES; ++k)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) z[q] += sums[k][quad][q];
+        }
+        if (part == 0 && u0 + quad < units) finish<DT, OT, 4>(p, o, e, m, n, left, z);
     }
 }
 
-// Whether a side can go straight to LDS: lines at multiples of 16 bytes, no partial chunk, 32-bit offsets
-// within a tile.
-inline bool direct_side(const void *p, int64_t line, int64_t out, int64_t sum, int64_t dense, int size) {
-    const int64_t e = 16 / size;
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && line % e == 0 && out % e == 0 && sum % e == 0 && dense % e == 0 &&
-           line >= 0 && line < (int64_t)1 << 21;
+// At most 16 MT rows of a (single tokens, small batches) against all of b: reading b once is all the work.  A
+// block takes 16 rows of b, its eight waves share the sum; both operands go from memory to registers as the
+// matrix instruction wants them, eight loads of b under way in each wave.
+constexpr int kFewWaves = 8;
+template <int DT, int OT, int MT>
+__global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(Product p) {
+    constexpr int SIZE = head_dtype_size(DT), E = 16 / SIZE, U = MT == 1 ? 8 : 4;
+    __shared__ f32x4 sums[kFewWaves][MT][64];
+    const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, q = lane % 16, g = lane / 16;
+    const int64_t tiles = (p.N + 15) / 16, units = tiles * p.out_batches;
+    const int64_t all = (p.K + 4 * E - 1) / (4 * E), from = all * wave / kFewWaves, to = all * (wave + 1) / kFewWaves;
+    for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+        const int64_t e = unit / tiles, n0 = unit % tiles * 16;
+        // rows behind the last one are read as the last one; their results are dropped
+        const elem_t<DT> *pb = static_cast<const elem_t<DT> *>(p.b) + e * p.b_out + (n0 + q < p.N ? n0 + q : p.N - 1) * p.b_n + g * E;
+        const elem_t<DT> *pa[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const int64_t m = t * 16 + q;
+            pa[t] = static_cast<const elem_t<DT> *>(p.a) + e * p.a_out + (m < p.M ? m : p.M - 1) * p.a_m + g * E;
+        }
+        const auto load = [&](const elem_t<DT> *line, int64_t step) {
+            const int64_t k = step * (4 * E), left = p.K - k - g * E;
+            i32x4 v = {0, 0, 0, 0};
+            if (left >= E) {
+                __builtin_memcpy(&v, line + k, 16);
+            } else if (left > 0) {
+                elem_t<DT> w[E];
+#pragma unroll
+                for (int x = 0; x < E; ++x) {
+                    w[x] = Elem<DT>::put(0.0f);
+                    if (x < left) w[x] = line[k + x];
+                }
+                __builtin_memcpy(&v, w, 16);
+            }
+            return v;
+        };
+        f32x4 acc[MT] = {};
+        int64_t step = from;
+        for (; step + U <= to && (step + U) * (4 * E) <= p.K; step += U) {
+            i32x4 b[U], a[MT][U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                __builtin_memcpy(&b[u], pb + (step + u) * (4 * E), 16);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) __builtin_memcpy(&a[t][u], pa[t] + (step + u) * (4 * E), 16);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) acc[t] = mma_chunk<DT>(b[u], a[t][u], acc[t]);
+        }
+        for (; step < to; ++step) {
+            const i32x4 b = load(pb, step);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[t] = mma_chunk<DT>(b, load(pa[t], step), acc[t]);
+        }
+        __syncthreads();   // the sums of the unit before have been read
+#pragma unroll
+        for (int t = 0; t < MT; ++t) sums[wave][t][lane] = acc[t];
+        __syncthreads();
+        if (wave < MT) {
+            f32x4 v = sums[0][wave][lane];
+#pragma unroll
+            for (int w = 1; w < kFewWaves; ++w) v += sums[w][wave][lane];
+            const int64_t m = wave * 16 + q, n = n0 + g * 4;
+            const int left = (int)(p.N - n < 4 ? p.N - n : 4);
+            float z[4] = {v[0], v[1], v[2], v[3]};
+            if (m < p.M && left > 0) finish<DT, OT, 4>(p, (e * p.M + m) * p.N + n, e, m, n, left, z);
+        }
+    }
 }
 
 template <int DT, int OT, bool IK, bool JK>
-void launch_tiles(Product p, hipStream_t st) {
-    const int size = head_dtype_size(DT);
-    const bool direct = direct_side(p.a, IK ? p.a_m : p.a_k, p.a_out, p.a_sum, IK ? p.K : p.M, size) &&
-                        direct_side(p.b, JK ? p.b_n : p.b_k, p.b_out, p.b_sum, JK ? p.K : p.N, size);
-    p.splits = 1;
-    p.part_steps = (p.K * size + 127) / 128 * p.sum_batches;
-    const auto tiles = [&](int bi, int bj) { return (p.M + bi - 1) / bi * ((p.N + bj - 1) / bj) * p.out_batches; };
+void launch_tiles(const Product &p, hipStream_t st) {
     const auto go = [&](auto bi, auto bj, auto wi, auto wj, auto d) {
-        k_tiles<DT, OT, IK, JK, bi.value, bj.value, wi.value, wj.value, d.value>
-            <<<blocks(tiles(bi.value, bj.value) * p.splits), wi.value * wj.value * 64, 0, st>>>(p);
+        const int64_t tiles = (p.M + bi.value - 1) / bi.value * ((p.N + bj.value - 1) / bj.value) * p.out_batches;
+        k_tiles<DT, OT, IK, JK, bi.value, bj.value, wi.value, wj.value, d.value><<<blocks(tiles * p.splits), wi.value * wj.value * 64, 0, st>>>(p);
     };
     using std::integral_constant;
+    const integral_constant<int, 1> one{};
     const integral_constant<int, 2> two{};
     const integral_constant<int, 4> four{};
-    const integral_constant<int, 128> small{};
+    const integral_constant<int, 64> narrow{};
+    const integral_constant<int, 128> mid{};
     const integral_constant<int, 256> big{};
-    if (p.M * p.N * p.out_batches == 0) return;
-    if (!direct) go(small, small, two, two, std::false_type{});
-    // two rounds of the large tile and more: 1177 against 1084 TFLOP/s at 8192^3 bf16; at one round (4096^3) they are equal
-    else if (DT != SSMAP_F32 && tiles(256, 256) >= 512) go(big, big, two, four, std::true_type{});
-    else go(small, small, two, two, std::true_type{});
+    if constexpr (DT != SSMAP_F32)
+        if (p.shape == kTileBig) return go(big, big, two, four, std::true_type{});
+    if (p.shape == kTileMid) go(mid, mid, two, two, std::true_type{});
+    else if (p.shape == kTileLow) go(narrow, big, one, four, std::true_type{});
+    else if (p.shape == kTileTall) go(big, narrow, four, one, std::true_type{});
+    else go(mid, mid, two, two, std::false_type{});
 }
 
 template <int DT, int OT>
 void launch_product(const Product &p, hipStream_t st) {
+    if (p.M * p.N * p.out_batches == 0) return;
+    if (p.shape == kFewRows) {
+        const unsigned n = blocks((p.N + 15) / 16 * p.out_batches);
+        if (p.M <= 16) k_few_rows<DT, OT, 1><<<n, kFewWaves * 64, 0, st>>>(p);
+        else k_few_rows<DT, OT, 2><<<n, kFewWaves * 64, 0, st>>>(p);
+        return;
+    }
     if (p.a_k == 1 && p.b_k == 1) launch_tiles<DT, OT, true, true>(p, st);
     else if constexpr (DT == OT) {
         if (p.a_k == 1) launch_tiles<DT, OT, true, false>(p, st);
         else launch_tiles<DT, OT, false, false>(p, st);
+    }
+    if (p.splits > 1) {
+        const int64_t quads = p.out_batches * p.M * ((p.N + 3) / 4);
+        if (p.splits >= 32) k_join_parts<DT, OT, 16><<<blocks((quads + 15) / 16), 256, 0, st>>>(p);
+        else k_join_parts<DT, OT, 1><<<blocks((quads + 255) / 256), 256, 0, st>>>(p);
     }
 }
 

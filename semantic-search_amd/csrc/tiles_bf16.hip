@@ -1,6 +1,5 @@
 // The matrix products of bfloat16 operands.
 #include <math.h>
-#include <stdlib.h>
 
 #include "tiles.h"
 

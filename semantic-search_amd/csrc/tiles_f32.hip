@@ -1,6 +1,5 @@
 // The matrix products of float32 operands.
 #include <math.h>
-#include <stdlib.h>
 
 #include "tiles.h"
 
