@@ -324,7 +324,7 @@ int64_t ssmap::plan_product(Product &p, int dtype) {
         p.shape = kTileMid;
     }
     // Fewer than half of the tiles that fit at once: the sum is split, in parts of eight stages at least
-    if (units && units * 2 <= full && steps >= 16) {
+    if (units && units <= 128 && steps >= 16) {
         const int64_t most = steps / 8, want = full / units < most ? full / units : most;
         p.part_steps = (steps + want - 1) / want;
         p.splits = (int)((steps + p.part_steps - 1) / p.part_steps);

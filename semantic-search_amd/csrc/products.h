@@ -19,7 +19,7 @@ struct Product {
     const void *bias, *res;
     int32_t bias_f32, bias_along_m, act, pad;
     int64_t res_out, res_m;
-    // the sum is split into `splits` parts of `part_steps` stages; more than one: float32 partial results go to
+    // the sum is split into `splits` parts of `part_steps` stages of 128 bytes a row; more than one: float32 partial results go to
     // parts[split][out_batches][M][N] and are joined afterwards
     int64_t part_steps;
     int32_t splits, shape;                  // shape: see plan_product

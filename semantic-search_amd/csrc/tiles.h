@@ -1,6 +1,6 @@
 // Matrix products on the matrix cores: out[m][n] = sum_k a(m, k) b(n, k), tile by tile.
 //
-// A block computes BI x BJ results, I the m side and J the n side, dense in memory.  A stage is 128 bytes of
+// A block computes BI x BJ results, I the m side and J the n side, dense in memory.  A stage is 128 of
 // every tile row in the sum's direction (64 values of 16 bits, 32 of float32), laid out in LDS as 16-byte
 // chunks; two stages alternate.  A side whose sum direction is dense in memory (KC) keeps its rows: chunk c
 // of row r sits at slot r * 8 + (c ^ (r & 7)), so that the 16 rows that one matrix instruction reads at one
@@ -40,19 +40,22 @@ __device__ __forceinline__ f32x4 mma_chunk(i32x4 j, i32x4 i, f32x4 acc) {
 
 constexpr uint32_t kNowhere = 0xFFFFFFF0u;   // a buffer offset behind every descriptor's end: reads as zero
 
-// One side of a tile: R rows (or columns) of it, NT threads.
-template <int DT, bool KC, int R, int NT>
+// One side of a tile: R rows (or columns) of it, C chunks of the sum's direction a stage, NT threads.
+template <int DT, bool KC, int R, int C, int NT>
 struct Side {
-    static constexpr int SIZE = head_dtype_size(DT), E = 16 / SIZE, KB = 128 / SIZE;   // values a chunk, a stage
-    static constexpr int PER = R * 8 / NT, ROW = R / E;                                // chunks a thread; a row (not KC)
-    static constexpr int BYTES = R * 128;
-    static_assert(R * 8 % NT == 0 && (KC || ROW >= 8), "tile shape");
+    static constexpr int SIZE = head_dtype_size(DT), E = 16 / SIZE, KB = C * E;   // values a chunk, a stage
+    static constexpr int PER = R * C / NT, ROW = R / E;                           // chunks a thread; a row (not KC)
+    static constexpr int BYTES = R * C * 16;
+    static_assert((C == 4 || C == 8) && R * C % NT == 0 && (KC || ROW >= 8), "tile shape");
 
     static __device__ __forceinline__ int swizzle(int k) { return DT == SSMAP_F32 ? ((k >> 2) & 3) << 2 : (k & 3) << 1; }
 
+    // KC: 128 bytes of consecutive slots hold eight rows' chunks of one c
+    static __device__ __forceinline__ int turn(int row) { return C == 8 ? row & 7 : (row >> 1) & 3; }
+
     // chunk of slot s: its row (KC) or sum index (not KC), and its place there
     static __device__ __forceinline__ void place(int s, int &line, int &c) {
-        if constexpr (KC) line = s / 8, c = (s % 8) ^ (line & 7);
+        if constexpr (KC) line = s / C, c = (s % C) ^ turn(line);
         else line = s / ROW, c = (s % ROW) ^ swizzle(line);
     }
     // how many of its values exist: `rows` are left on this side, `ks` in the sum
@@ -117,7 +120,7 @@ struct Side {
     static __device__ __forceinline__ i32x4 read(const char *lds, int row0, int kk) {
         const int lane = threadIdx.x % 64, q = lane % 16, g = lane / 16;
         if constexpr (KC) {
-            return *reinterpret_cast<const i32x4 *>(lds + (row0 + q) * 128 + (((kk * 4 + g) ^ (q & 7)) * 16));
+            return *reinterpret_cast<const i32x4 *>(lds + (row0 + q) * (C * 16) + (((kk * 4 + g) ^ turn(q)) * 16));
         } else if constexpr (DT == SSMAP_F32) {
             f32x4 v;
             const int i = row0 + q;
@@ -201,18 +204,19 @@ __device__ __forceinline__ void finish(const Product &p, int64_t o, int64_t e, i
     put(O{}, p.out);
 }
 
-// BI x BJ results a block, WI x WJ waves.  DIRECT: both sides go straight to LDS (see Side::fetch).
-template <int DT, int OT, bool IK, bool JK, int BI, int BJ, int WI, int WJ, bool DIRECT>
+// BI x BJ results a block, WI x WJ waves, stages of C chunks in NBUF buffers.  DIRECT: both sides go straight to
+// LDS (see Side::fetch), NBUF - 1 stages ahead; otherwise through registers, one stage ahead.
+template <int DT, int OT, bool IK, bool JK, int BI, int BJ, int WI, int WJ, int C, int NBUF, bool DIRECT>
 __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
     constexpr int NT = WI * WJ * 64, TI = BI / WI / 16, TJ = BJ / WJ / 16, SIZE = head_dtype_size(DT);
-    using I = Side<DT, IK, BI, NT>;
-    using J = Side<DT, JK, BJ, NT>;
+    using I = Side<DT, IK, BI, C, NT>;
+    using J = Side<DT, JK, BJ, C, NT>;
     constexpr int PITCH = TJ * 16 + 4;                 // floats a row while results are turned: four off, for the banks
     constexpr int HI = TI > 4 ? TI / 2 : TI;           // rows of 16 turned at once
     constexpr int STAGE = I::BYTES + J::BYTES, TURN = WI * WJ * HI * 16 * PITCH * 4;
-    __shared__ __attribute__((aligned(1024))) char lds_all[2 * STAGE > TURN ? 2 * STAGE : TURN];
+    __shared__ __attribute__((aligned(1024))) char lds_all[NBUF * STAGE > TURN ? NBUF * STAGE : TURN];
     const auto stage = [&](int buf) { return lds_all + buf * STAGE; };
-    const int wave = threadIdx.x / 64, wi = wave % WI, wj = wave / WI;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wi = wave % WI, wj = wave / WI;
     const int64_t tiles_m = (p.M + BI - 1) / BI, tiles_n = (p.N + BJ - 1) / BJ, tiles = tiles_m * tiles_n;
     const int64_t steps = (p.K + I::KB - 1) / I::KB, all_steps = steps * p.sum_batches;
     const int64_t units = tiles * p.out_batches * p.splits;
@@ -227,7 +231,8 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
         const int64_t in_band = tile % (BAND * tiles_n);
         const int64_t i0 = (band * BAND + in_band % rows_in) * BI, j0 = in_band / rows_in * BJ;
         const int rows_i = (int)(p.M - i0 < BI ? p.M - i0 : BI), rows_j = (int)(p.N - j0 < BJ ? p.N - j0 : BJ);
-        const int64_t first = split * p.part_steps, last = first + p.part_steps < all_steps ? first + p.part_steps : all_steps;
+        const int64_t part = p.part_steps * (8 / C);   // planned in stages of eight chunks
+        const int64_t first = split * part, last = first + part < all_steps ? first + part : all_steps;
         const int64_t ld_i = (IK ? p.a_m : p.a_k) * SIZE, ld_j = (JK ? p.b_n : p.b_k) * SIZE;
         const int64_t step_i = (IK ? 1 : p.a_k) * (int64_t)(I::KB * SIZE), step_j = (JK ? 1 : p.b_k) * (int64_t)(I::KB * SIZE);
         const char *pa = static_cast<const char *>(p.a) + (e * p.a_out + i0 * p.a_m) * SIZE;
@@ -279,32 +284,98 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
             }
         };
         f32x4 acc[TI][TJ] = {};
-        if (first < last) {
-            fetch(0);
-            keep(0);
-        }
-        for (int64_t t = first; t < last; ++t) {
-            const int buf = (int)((t - first) & 1);
-            // this wave's part of the stage has landed; behind the barrier everybody's has, and nobody reads
-            // the other buffer any more
-            if constexpr (DIRECT) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            __syncthreads();
-            const bool more = t + 1 < last;
-            if (more) fetch(buf ^ 1);
+        i32x4 fi[TI], fj[TJ];
+        const auto read = [&](int buf, int kk) {
             const char *li = stage(buf), *lj = li + I::BYTES;
 #pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                i32x4 fi[TI], fj[TJ];
+            for (int i = 0; i < TI; ++i) fi[i] = I::read(li, (wi * TI + i) * 16, kk);
 #pragma unroll
-                for (int i = 0; i < TI; ++i) fi[i] = I::read(li, (wi * TI + i) * 16, kk);
+            for (int j = 0; j < TJ; ++j) fj[j] = J::read(lj, (wj * TJ + j) * 16, kk);
+        };
+        const auto multiply = [&] {
 #pragma unroll
-                for (int j = 0; j < TJ; ++j) fj[j] = J::read(lj, (wj * TJ + j) * 16, kk);
+            for (int i = 0; i < TI; ++i)
 #pragma unroll
-                for (int i = 0; i < TI; ++i)
-#pragma unroll
-                    for (int j = 0; j < TJ; ++j) acc[i][j] = mma_chunk<DT>(fj[j], fi[i], acc[i][j]);
+                for (int j = 0; j < TJ; ++j) acc[i][j] = mma_chunk<DT>(fj[j], fi[i], acc[i][j]);
+        };
+        if constexpr (WI * WJ == 8) {
+            // Two waves a SIMD take turns: while one multiplies half a stage, the other reads its next half from
+            // LDS.  The second four waves run one turn behind.  A barrier ends each turn; the scheduler moves
+            // nothing over it.  With turns 4t ... 4t + 3 of the first waves for stage t (read, multiply, read,
+            // multiply), the second waves read stage t for the last time in turn 4t + 3: in turn 4t + 4 both send
+            // for stage t + 2, into the same buffer, and at the end of turn 4t + 7 both have waited for it.
+            static_assert(DIRECT && C == 8 && NBUF == 2, "two turns a stage");
+            const bool late = wave >= 4;
+            const auto turn_ends = [&] {
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            const auto have_read = [&] { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); };
+            const auto have_landed = [&] { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
+            if (first < last) {
+                fetch(0);
+                have_landed();
+                turn_ends();
+                if (late) {
+                    if (first + 1 < last) fetch(1);
+                    turn_ends();
+                }
+                for (int64_t t = first; t < last; ++t) {
+                    const int buf = (int)((t - first) & 1);
+                    if (!late && t + 1 < last) fetch(buf ^ 1);
+                    read(buf, 0);
+                    have_read();
+                    turn_ends();
+                    __builtin_amdgcn_s_setprio(1);
+                    multiply();
+                    __builtin_amdgcn_s_setprio(0);
+                    turn_ends();
+                    read(buf, 1);
+                    if (late) have_landed();
+                    have_read();
+                    turn_ends();
+                    if (late && t + 2 < last) fetch(buf);
+                    __builtin_amdgcn_s_setprio(1);
+                    multiply();
+                    __builtin_amdgcn_s_setprio(0);
+                    if (!late) have_landed();
+                    turn_ends();
+                }
+                if (!late) turn_ends();   // the second waves' last turn
             }
-            if (more) keep(buf ^ 1);
+        } else {
+            static_assert(DIRECT || NBUF == 2, "one stage of registers");
+            int64_t sent = first;
+            for (; sent < first + NBUF - 1 && sent < last; ++sent) {
+                fetch((int)(sent - first));
+                keep((int)(sent - first));
+            }
+            int buf = 0;
+            for (int64_t t = first; t < last; ++t) {
+                // This wave's part of the stage has landed (loads return in order: those of the stages behind it may
+                // be under way), and its reads of the stage before have; behind the barrier that holds for all, and
+                // the buffer of the stage before is free.
+                if constexpr (DIRECT) {
+                    if (sent < last) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NBUF - 2) * (I::PER + J::PER)) : "memory");
+                    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("" ::: "memory");
+                } else {
+                    __syncthreads();
+                }
+                const int next = buf ? buf - 1 : NBUF - 1;
+                const bool more = sent < last;
+                if (more) fetch(next), ++sent;
+#pragma unroll
+                for (int kk = 0; kk < C / 4; ++kk) {
+                    read(buf, kk);
+                    multiply();
+                }
+                if (more) keep(next);
+                buf = buf + 1 == NBUF ? 0 : buf + 1;
+            }
         }
         __syncthreads();   // nobody reads the stages any more
         // Each wave turns its own results round in LDS, HI rows of 16 at a time: out of the registers with four
@@ -462,23 +533,24 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(Product p) {
 
 template <int DT, int OT, bool IK, bool JK>
 void launch_tiles(const Product &p, hipStream_t st) {
-    const auto go = [&](auto bi, auto bj, auto wi, auto wj, auto d) {
+    const auto go = [&](auto bi, auto bj, auto wi, auto wj, auto c, auto nbuf, auto d) {
         const int64_t tiles = (p.M + bi.value - 1) / bi.value * ((p.N + bj.value - 1) / bj.value) * p.out_batches;
-        k_tiles<DT, OT, IK, JK, bi.value, bj.value, wi.value, wj.value, d.value><<<blocks(tiles * p.splits), wi.value * wj.value * 64, 0, st>>>(p);
+        k_tiles<DT, OT, IK, JK, bi.value, bj.value, wi.value, wj.value, c.value, nbuf.value, d.value><<<blocks(tiles * p.splits), wi.value * wj.value * 64, 0, st>>>(p);
     };
     using std::integral_constant;
     const integral_constant<int, 1> one{};
     const integral_constant<int, 2> two{};
     const integral_constant<int, 4> four{};
+    const integral_constant<int, 8> eight{};
     const integral_constant<int, 64> narrow{};
     const integral_constant<int, 128> mid{};
     const integral_constant<int, 256> big{};
     if constexpr (DT != SSMAP_F32)
-        if (p.shape == kTileBig) return go(big, big, two, four, std::true_type{});
-    if (p.shape == kTileMid) go(mid, mid, two, two, std::true_type{});
-    else if (p.shape == kTileLow) go(narrow, big, one, four, std::true_type{});
-    else if (p.shape == kTileTall) go(big, narrow, four, one, std::true_type{});
-    else go(mid, mid, two, two, std::false_type{});
+        if (p.shape == kTileBig) return go(big, big, two, four, eight, two, std::true_type{});
+    if (p.shape == kTileMid) go(mid, mid, two, two, eight, two, std::true_type{});
+    else if (p.shape == kTileLow) go(narrow, big, one, four, eight, two, std::true_type{});
+    else if (p.shape == kTileTall) go(big, narrow, four, one, eight, two, std::true_type{});
+    else go(mid, mid, two, two, eight, two, std::false_type{});
 }
 
 template <int DT, int OT>

@@ -473,6 +473,32 @@ def test_linear_planes(lead, K, N, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("n,K,N", [(8190, 200, 4088), (16400, 64, 2056), (4096, 1000, 8190), (40000, 128, 48), (2000, 2048, 1500), (100, 8200, 600)])
+def test_linear_large(n, K, N, dtype):
+    """Sizes that take the largest tiles, split sums and many tiles with partial ones at the ends; forward and
+    backward against 64-bit products on the GPU."""
+    g = torch.Generator(device="cuda").manual_seed(n + K)
+    x = torch.randn((n, K), device="cuda", generator=g).to(dtype)
+    w = (torch.randn((N, K), device="cuda", generator=g) / math.sqrt(K)).to(dtype)
+    b = torch.randn(N, device="cuda", generator=g)
+    xd, wd = x.double(), w.double()
+
+    def check(name, got, want, size, terms, extra=0.0):
+        tol = (U * (terms + 8) + extra) * size * 1.0001 + HALF[dtype] * want.abs() * 1.0001 + SMALLEST[dtype]
+        off = (got.double() - want).abs() - tol
+        assert float(off.max()) <= 0, f"{name}: off by {float(off.max())} over the tolerance"
+
+    size = xd.abs() @ wd.abs().t()
+    check("y", ssa.linear(x, w, b), xd @ wd.t() + b.double(), size + b.double().abs(), K)
+    dy = torch.randn((n, N), device="cuda", generator=g).to(dtype)
+    got = ssa.linear_grad(dy, x, w)
+    d = dy.double()
+    check("gradient of x", got.x, d @ wd, d.abs() @ wd.abs(), N)
+    check("gradient of weight", got.weight, d.t() @ xd, d.abs().t() @ xd.abs(), n)
+    check("gradient of bias", got.bias, d.sum(0), d.abs().sum(0), n)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
 def test_linear_views(dtype):
     """Rows of wider tensors, odd starts, expanded residuals; NaN beside what may be read."""
     for K, N, n in ((40, 24, 6), (67, 33, 40), (256, 64, 3), (264, 136, 200)):
