@@ -50,8 +50,10 @@ __device__ __forceinline__ void dz_pack(const elem_t<OT> *g, const elem_t<DT> *p
             for (int e = 0; e < 8; ++e)
                 if (e < left) z[e] = Elem<DT>::get(pre[e]);
         }
+        with_activation(act, [&](auto a) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= slope<DT == SSMAP_F32>(z[e], act);
+            for (int e = 0; e < 8; ++e) v[e] *= slope<a.value, DT == SSMAP_F32>(z[e]);
+        });
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) sum[e] += v[e];
@@ -81,7 +83,8 @@ __global__ __launch_bounds__(256) void k_dz_rows(int64_t batch, int64_t rows, in
         const int left = (int)(outer - n < 8 ? outer - n : 8);
         float sum[8] = {};
         if (left > 0)
-            for (int64_t r = r0 + ty; r < r0 + kDzRows && r < rows; r += 8) {
+#pragma unroll 4
+            for (int64_t r = r0 + ty; r < (r0 + kDzRows < rows ? r0 + kDzRows : rows); r += 8) {
                 const int64_t o = (b * rows + r) * outer + n;
                 dz_pack<DT, OT>(g + b * g_batch + r * g_row + n, pre ? pre + o : nullptr, dz ? dz + o : nullptr, left, act, sum);
             }
@@ -315,16 +318,16 @@ int64_t ssmap::plan_product(Product &p, int dtype) {
     } else if (p.N <= 64) {
         p.shape = kTileTall;
         units = tiles(256, 64);
-    } else if (dtype != SSMAP_F32 && tiles(256, 256) >= 512) {
-        // two rounds of the large tile and more: 1177 against 1084 TFLOP/s at 8192^3 bf16; at one round (4096^3)
-        // they are equal
+    } else if (dtype != SSMAP_F32 && tiles(256, 256) >= 192) {
+        // three quarters of a round of the large tile and more: 112 against 127 us at 4096^3 bf16 (256 tiles)
         p.shape = kTileBig;
         units = tiles(256, 256), full = 256;
     } else {
         p.shape = kTileMid;
     }
-    // Fewer than half of the tiles that fit at once: the sum is split, in parts of eight stages at least
-    if (units && units <= 128 && steps >= 16) {
+    // Few tiles: the sum is split, in parts of eight stages at least (up to 128 tiles); with half of the tiles that
+    // fit at once only a long sum (2048 x 2048 from 8192 products, bf16: 112 -> 95 us; from 2048: 33 -> 42)
+    if (units && (units <= 128 ? steps >= 16 : units * 2 <= full && steps >= 96)) {
         const int64_t most = steps / 8, want = full / units < most ? full / units : most;
         p.part_steps = (steps + want - 1) / want;
         p.splits = (int)((steps + p.part_steps - 1) / p.part_steps);

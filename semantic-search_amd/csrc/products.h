@@ -3,6 +3,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "heads.h"
 
 namespace ssmap {
@@ -49,36 +51,41 @@ __device__ __forceinline__ float logistic(float x) {    // 1 / (1 + exp(-x))
     if constexpr (FINE) return 1.0f / (1.0f + expf(-x));
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * x));
 }
-template <bool FINE>
-__device__ __forceinline__ float activate(float z, int act) {
-    if (act == SSMAP_ACT_RELU) return z < 0.0f ? 0.0f : z;
-    if (act == SSMAP_ACT_GELU) return z * half_erfc<FINE>(-0.70710678118654752f * z);
-    if (act == SSMAP_ACT_GELU_TANH) {
-        // (1 + tanh u) / 2 = 1 / (1 + exp(-2u))
-        return z * logistic<FINE>(1.5957691216057308f * (z + 0.044715f * z * z * z));
-    }
-    if (act == SSMAP_ACT_SILU) return z * logistic<FINE>(z);
+template <int ACT, bool FINE>
+__device__ __forceinline__ float activate(float z) {
+    if constexpr (ACT == SSMAP_ACT_RELU) return z < 0.0f ? 0.0f : z;
+    if constexpr (ACT == SSMAP_ACT_GELU) return z * half_erfc<FINE>(-0.70710678118654752f * z);
+    // (1 + tanh u) / 2 = 1 / (1 + exp(-2u))
+    if constexpr (ACT == SSMAP_ACT_GELU_TANH) return z * logistic<FINE>(1.5957691216057308f * (z + 0.044715f * z * z * z));
+    if constexpr (ACT == SSMAP_ACT_SILU) return z * logistic<FINE>(z);
     return z;
 }
-
-template <bool FINE>
-__device__ __forceinline__ float slope(float z, int act) {
-    if (act == SSMAP_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
-    if (act == SSMAP_ACT_GELU) {
+template <int ACT, bool FINE>
+__device__ __forceinline__ float slope(float z) {
+    if constexpr (ACT == SSMAP_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+    if constexpr (ACT == SSMAP_ACT_GELU) {
         const float bell = FINE ? expf(-0.5f * z * z) : __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
         return half_erfc<FINE>(-0.70710678118654752f * z) + z * 0.39894228040143268f * bell;
     }
-    if (act == SSMAP_ACT_GELU_TANH) {
+    if constexpr (ACT == SSMAP_ACT_GELU_TANH) {
         // q = (1 + tanh u) / 2; its slope in u is 2 q (1 - q), which is 0 where z may be infinite
         const float q = logistic<FINE>(1.5957691216057308f * (z + 0.044715f * z * z * z));
         const float du = 0.79788456080286536f * (1.0f + 3.0f * 0.044715f * z * z);
         return q + (q > 0.0f && q < 1.0f ? z * 2.0f * q * (1.0f - q) * du : 0.0f);
     }
-    if (act == SSMAP_ACT_SILU) {
+    if constexpr (ACT == SSMAP_ACT_SILU) {
         const float q = logistic<FINE>(z);
         return q + (q > 0.0f && q < 1.0f ? z * q * (1.0f - q) : 0.0f);
     }
     return 1.0f;
+}
+// Calls f with the activation as a constant: one branch for a run of values, not one for each.
+template <typename F>
+__device__ __forceinline__ void with_activation(int act, F f) {
+    if (act == SSMAP_ACT_RELU) f(std::integral_constant<int, SSMAP_ACT_RELU>{});
+    else if (act == SSMAP_ACT_GELU) f(std::integral_constant<int, SSMAP_ACT_GELU>{});
+    else if (act == SSMAP_ACT_GELU_TANH) f(std::integral_constant<int, SSMAP_ACT_GELU_TANH>{});
+    else if (act == SSMAP_ACT_SILU) f(std::integral_constant<int, SSMAP_ACT_SILU>{});
 }
 
 // Enqueues a planned product of operands of type DT with results of type OT (DT or SSMAP_F32).

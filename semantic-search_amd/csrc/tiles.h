@@ -146,62 +146,88 @@ struct Side {
     }
 };
 
-// N results next to each other (n, n + 1, ...), of which `left` exist.  `o` is the first one's place in the
-// dense output.
-template <int DT, int OT, int N>
-__device__ __forceinline__ void finish(const Product &p, int64_t o, int64_t e, int64_t m, int64_t n, int left, float (&z)[N]) {
-    const auto each = [&](auto f) {
+// N values next to each other, of which `left` exist; WHOLE: all of them, which the caller knows for its whole
+// wave (with a branch for each lane the compiler merges both ways into pieces: 1108 against 1359 us at 8192^3
+// in 128 wide tiles).
+template <int DT, int N>
+struct Run {
+    elem_t<DT> v[N];
+};
+template <bool WHOLE, int DT, int N>
+__device__ __forceinline__ Run<DT, N> load_run(const void *from, int64_t at, int left) {
+    const elem_t<DT> *src = static_cast<const elem_t<DT> *>(from) + at;
+    Run<DT, N> r;
+    if constexpr (WHOLE) {
+        __builtin_memcpy(&r, src, sizeof r);
+    } else {
+#pragma unroll
+        for (int q = 0; q < N; ++q) {
+            r.v[q] = Elem<DT>::put(0.0f);
+            if (q < left) r.v[q] = src[q];
+        }
+    }
+    return r;
+}
+template <bool WHOLE, int DT, int N>
+__device__ __forceinline__ void store_run(void *to, int64_t at, int left, const float (&z)[N]) {
+    elem_t<DT> *dst = static_cast<elem_t<DT> *>(to) + at;
+    Run<DT, N> r;
+#pragma unroll
+    for (int q = 0; q < N; ++q) r.v[q] = Elem<DT>::put(z[q]);
+    if constexpr (WHOLE) {
+        __builtin_memcpy(dst, &r, sizeof r);
+    } else {
 #pragma unroll
         for (int q = 0; q < N; ++q)
-            if (q < left) f(q);
-    };
-    const auto get = [&](auto tag, const void *from, int64_t at, float (&v)[N]) {
-        constexpr int T = decltype(tag)::value;
-        const elem_t<T> *src = static_cast<const elem_t<T> *>(from) + at;
-        if (left >= N) {
-            elem_t<T> w[N];
-            __builtin_memcpy(w, src, sizeof w);
+            if (q < left) dst[q] = r.v[q];
+    }
+}
+
+// The epilogue's operands of N results at (m, n ... n + N - 1).
+template <bool WHOLE, int DT, int N>
+__device__ __forceinline__ void load_bias(const Product &p, int64_t m, int64_t n, int left, float (&b)[N]) {
 #pragma unroll
-            for (int q = 0; q < N; ++q) v[q] = Elem<T>::get(w[q]);
-        } else {
-            each([&](int q) { v[q] = Elem<T>::get(src[q]); });
-        }
-    };
-    const auto put = [&](auto tag, void *to) {
-        constexpr int T = decltype(tag)::value;
-        elem_t<T> *dst = static_cast<elem_t<T> *>(to) + o, w[N];
+    for (int q = 0; q < N; ++q) b[q] = 0.0f;
+    if (!p.bias) return;
+    if (p.bias_along_m) {
+        const float v = p.bias_f32 ? static_cast<const float *>(p.bias)[m] : Elem<DT>::get(static_cast<const elem_t<DT> *>(p.bias)[m]);
 #pragma unroll
-        for (int q = 0; q < N; ++q) w[q] = Elem<T>::put(z[q]);
-        if (left >= N) __builtin_memcpy(dst, w, sizeof w);
-        else each([&](int q) { dst[q] = w[q]; });
-    };
-    using D = std::integral_constant<int, DT>;
-    using O = std::integral_constant<int, OT>;
-    using F = std::integral_constant<int, SSMAP_F32>;
-    float v[N] = {};
+        for (int q = 0; q < N; ++q) b[q] = v;
+    } else if (p.bias_f32) {
+        const Run<SSMAP_F32, N> r = load_run<WHOLE, SSMAP_F32, N>(p.bias, n, left);
+#pragma unroll
+        for (int q = 0; q < N; ++q) b[q] = r.v[q];
+    } else {
+        const Run<DT, N> r = load_run<WHOLE, DT, N>(p.bias, n, left);
+#pragma unroll
+        for (int q = 0; q < N; ++q) b[q] = Elem<DT>::get(r.v[q]);
+    }
+}
+// `o` is the first result's place in the dense output.
+template <bool WHOLE, int DT, int OT, int N>
+__device__ __forceinline__ void finish(const Product &p, int64_t o, int left, float (&z)[N], const float (&bias)[N], const Run<OT, N> &res) {
     if (p.bias) {
-        if (p.bias_along_m) {
-            const float b = p.bias_f32 ? static_cast<const float *>(p.bias)[m] : Elem<DT>::get(static_cast<const elem_t<DT> *>(p.bias)[m]);
 #pragma unroll
-            for (int q = 0; q < N; ++q) z[q] += b;
-        } else {
-            if (p.bias_f32) get(F{}, p.bias, n, v);
-            else get(D{}, p.bias, n, v);
-#pragma unroll
-            for (int q = 0; q < N; ++q) z[q] += v[q];
-        }
+        for (int q = 0; q < N; ++q) z[q] += bias[q];
     }
-    if (p.pre) put(D{}, p.pre);
-    if (p.act) {
+    if (p.pre) store_run<WHOLE, DT, N>(p.pre, o, left, z);
+    with_activation(p.act, [&](auto act) {
 #pragma unroll
-        for (int q = 0; q < N; ++q) z[q] = activate<OT == SSMAP_F32>(z[q], p.act);
-    }
+        for (int q = 0; q < N; ++q) z[q] = activate<act.value, OT == SSMAP_F32>(z[q]);
+    });
     if (p.res) {
-        get(O{}, p.res, e * p.res_out + m * p.res_m + n, v);
 #pragma unroll
-        for (int q = 0; q < N; ++q) z[q] += v[q];
+        for (int q = 0; q < N; ++q) z[q] += Elem<OT>::get(res.v[q]);
     }
-    put(O{}, p.out);
+    store_run<WHOLE, OT, N>(p.out, o, left, z);
+}
+template <bool WHOLE, int DT, int OT, int N>
+__device__ __forceinline__ void finish_at(const Product &p, int64_t e, int64_t m, int64_t n, int left, float (&z)[N]) {
+    float bias[N];
+    load_bias<WHOLE, DT, N>(p, m, n, left, bias);
+    Run<OT, N> res;
+    if (p.res) res = load_run<WHOLE, OT, N>(p.res, e * p.res_out + m * p.res_m + n, left);
+    finish<WHOLE, DT, OT, N>(p, (e * p.M + m) * p.N + n, left, z, bias, res);
 }
 
 // BI x BJ results a block, WI x WJ waves, stages of C chunks in NBUF buffers.  DIRECT: both sides go straight to
@@ -213,6 +239,7 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
     using J = Side<DT, JK, BJ, C, NT>;
     constexpr int PITCH = TJ * 16 + 4;                 // floats a row while results are turned: four off, for the banks
     constexpr int HI = TI > 4 ? TI / 2 : TI;           // rows of 16 turned at once
+    constexpr int LINE = TJ * 16 / 8, ROWS = 64 / LINE;   // lanes a row, rows at once
     constexpr int STAGE = I::BYTES + J::BYTES, TURN = WI * WJ * HI * 16 * PITCH * 4;
     __shared__ __attribute__((aligned(1024))) char lds_all[NBUF * STAGE > TURN ? NBUF * STAGE : TURN];
     const auto stage = [&](int buf) { return lds_all + buf * STAGE; };
@@ -300,10 +327,13 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
         };
         if constexpr (WI * WJ == 8) {
             // Two waves a SIMD take turns: while one multiplies half a stage, the other reads its next half from
-            // LDS.  The second four waves run one turn behind.  A barrier ends each turn; the scheduler moves
-            // nothing over it.  With turns 4t ... 4t + 3 of the first waves for stage t (read, multiply, read,
-            // multiply), the second waves read stage t for the last time in turn 4t + 3: in turn 4t + 4 both send
-            // for stage t + 2, into the same buffer, and at the end of turn 4t + 7 both have waited for it.
+            // LDS and sends for the stage after the next.  The second four waves run one turn behind.  A barrier
+            // ends each turn; the scheduler moves nothing over it.  The first waves read the halves of stage t in
+            // turns 4t and 4t + 2 and multiply them in the turns behind; the second waves read the last half of
+            // stage t - 1 in turn 4t - 1.  So from turn 4t on that stage's buffer is free for stage t + 1: the
+            // first waves send for it in turn 4t, the second ones in turn 4t + 1, each behind its reads (in front
+            // of them or of the matrix instructions the queue of loads held those up: 978 against 922 us at
+            // 8192^3), and all have waited for it at the end of turn 4t + 3.
             static_assert(DIRECT && C == 8 && NBUF == 2, "two turns a stage");
             const bool late = wave >= 4;
             const auto turn_ends = [&] {
@@ -318,14 +348,12 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
                 fetch(0);
                 have_landed();
                 turn_ends();
-                if (late) {
-                    if (first + 1 < last) fetch(1);
-                    turn_ends();
-                }
+                if (late) turn_ends();
                 for (int64_t t = first; t < last; ++t) {
                     const int buf = (int)((t - first) & 1);
-                    if (!late && t + 1 < last) fetch(buf ^ 1);
                     read(buf, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (t + 1 < last) fetch(buf ^ 1);
                     have_read();
                     turn_ends();
                     __builtin_amdgcn_s_setprio(1);
@@ -336,7 +364,6 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
                     if (late) have_landed();
                     have_read();
                     turn_ends();
-                    if (late && t + 2 < last) fetch(buf);
                     __builtin_amdgcn_s_setprio(1);
                     multiply();
                     __builtin_amdgcn_s_setprio(0);
@@ -379,37 +406,57 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
         }
         __syncthreads();   // nobody reads the stages any more
         // Each wave turns its own results round in LDS, HI rows of 16 at a time: out of the registers with four
-        // neighbouring n a lane, back with eight, so that the epilogue is one loop over whole rows.
+        // neighbouring n a lane, back with eight.  Loops stay loops here: the code runs once a tile, and
+        // unrolled it costs more in instruction fetches than the whole epilogue (112 of 537 us at 8192 x 4096 x
+        // 8192).  The residual of the next rows is under way while these are finished.
         const int lane = threadIdx.x % 64, q = lane % 16, g = lane / 16;
         float *turn = reinterpret_cast<float *>(lds_all + wave * (HI * 16 * PITCH * 4));
-#pragma unroll
+        const int col = lane % LINE * 8;
+        const int64_t n = j0 + wj * TJ * 16 + col;
+        const float *mine = turn + lane / LINE * PITCH + col;
+        const bool whole = rows_i == BI && rows_j == BJ;
+#pragma unroll 1
         for (int h = 0; h < TI / HI; ++h) {
 #pragma unroll
-            for (int i = 0; i < HI; ++i)
+            for (int k = 0; k < TI / HI; ++k)
+                if (k == h)
 #pragma unroll
-                for (int j = 0; j < TJ; ++j) *reinterpret_cast<f32x4 *>(turn + (i * 16 + q) * PITCH + j * 16 + g * 4) = acc[h * HI + i][j];
+                    for (int i = 0; i < HI; ++i)
+#pragma unroll
+                        for (int j = 0; j < TJ; ++j) *reinterpret_cast<f32x4 *>(turn + (i * 16 + q) * PITCH + j * 16 + g * 4) = acc[k * HI + i][j];
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");   // the wave's own writes, in order
             __builtin_amdgcn_wave_barrier();
-            constexpr int LINE = TJ * 16 / 8;   // lanes a row
+            int64_t m = i0 + (wi * TI + h * HI) * 16 + lane / LINE;
+            if (whole) {
+                float bias[8];
+                load_bias<true, DT, 8>(p, m, n, 8, bias);
+                Run<OT, 8> res, next;
+                int64_t o = (e * p.M + m) * p.N + n;
+                if (p.res) next = load_run<true, OT, 8>(p.res, e * p.res_out + m * p.res_m + n, 8);
 #pragma unroll 1
-            for (int u = lane; u < HI * 16 * LINE; u += 64) {
-                const int row = u / LINE, col = u % LINE * 8;
-                const int64_t m = i0 + (wi * TI + h * HI) * 16 + row, n = j0 + wj * TJ * 16 + col;
-                const int left = (int)(p.N - n < 8 ? p.N - n : 8);
-                if (m >= p.M || left <= 0) continue;
-                const int64_t o = (e * p.M + m) * p.N + n;
-                float z[8];
-                __builtin_memcpy(z, turn + row * PITCH + col, 32);
-                if (p.splits > 1) {
-                    float *part = p.parts + split * p.out_batches * p.M * p.N + o;
-                    if (left == 8) __builtin_memcpy(part, z, 32);
-                    else {
-#pragma unroll
-                        for (int s = 0; s < 8; ++s)
-                            if (s < left) part[s] = z[s];
+                for (int r0 = 0; r0 < HI * 16; r0 += ROWS) {
+                    res = next;
+                    if (p.res && r0 + ROWS < HI * 16) next = load_run<true, OT, 8>(p.res, e * p.res_out + (m + ROWS) * p.res_m + n, 8);
+                    float z[8];
+                    __builtin_memcpy(z, __builtin_assume_aligned(mine + r0 * PITCH, 16), 32);
+                    if (p.splits > 1) {
+                        store_run<true, SSMAP_F32, 8>(p.parts + split * p.out_batches * p.M * p.N, o, 8, z);
+                    } else {
+                        if (p.bias_along_m) load_bias<true, DT, 8>(p, m, n, 8, bias);
+                        finish<true, DT, OT, 8>(p, o, 8, z, bias, res);
                     }
-                } else {
-                    finish<DT, OT, 8>(p, o, e, m, n, left, z);
+                    m += ROWS;
+                    o += ROWS * p.N;
+                }
+            } else {
+                const int left = (int)(p.N - n < 8 ? p.N - n : 8);
+#pragma unroll 1
+                for (int r0 = 0; r0 < HI * 16; r0 += ROWS, m += ROWS) {
+                    if (m >= p.M || left <= 0) continue;
+                    float z[8];
+                    __builtin_memcpy(z, __builtin_assume_aligned(mine + r0 * PITCH, 16), 32);
+                    if (p.splits > 1) store_run<false, SSMAP_F32, 8>(p.parts + split * p.out_batches * p.M * p.N, (e * p.M + m) * p.N + n, left, z);
+                    else finish_at<false, DT, OT, 8>(p, e, m, n, left, z);
                 }
             }
             __builtin_amdgcn_wave_barrier();
@@ -454,7 +501,10 @@ __global__ __launch_bounds__(256) void k_join_parts(Product p) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) z[q] += sums[k][quad][q];
         }
-        if (part == 0 && u0 + quad < units) finish<DT, OT, 4>(p, o, e, m, n, left, z);
+        if (part == 0 && u0 + quad < units) {
+            if (left == 4) finish_at<true, DT, OT, 4>(p, e, m, n, 4, z);
+            else finish_at<false, DT, OT, 4>(p, e, m, n, left, z);
+        }
     }
 }
 
@@ -526,7 +576,10 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(Product p) {
             const int64_t m = wave * 16 + q, n = n0 + g * 4;
             const int left = (int)(p.N - n < 4 ? p.N - n : 4);
             float z[4] = {v[0], v[1], v[2], v[3]};
-            if (m < p.M && left > 0) finish<DT, OT, 4>(p, (e * p.M + m) * p.N + n, e, m, n, left, z);
+            if (m < p.M && left > 0) {
+            if (left == 4) finish_at<true, DT, OT, 4>(p, e, m, n, 4, z);
+            else finish_at<false, DT, OT, 4>(p, e, m, n, left, z);
+        }
         }
     }
 }
