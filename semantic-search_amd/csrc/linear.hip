@@ -305,12 +305,21 @@ int64_t ssmap::plan_product(Product &p, int dtype) {
     const bool direct = direct_side(p.a, ik ? p.a_m : p.a_k, p.a_out, p.a_sum, ik ? p.K : p.M, size) &&
                         direct_side(p.b, jk ? p.b_n : p.b_k, p.b_out, p.b_sum, jk ? p.K : p.N, size);
     const auto tiles = [&](int bi, int bj) { return (p.M + bi - 1) / bi * ((p.N + bj - 1) / bj) * p.out_batches; };
+    const int64_t e = 16 / size;
+    if (p.M <= kHeadMost && ik && jk && p.sum_batches == 1 && p.a_out == 0 && p.K >= e && p.K % e == 0 && head_bytes(p, size) <= kHeadBytes &&
+        p.N * p.out_batches >= 16384) {
+        p.shape = kHead;
+        return 0;
+    }
     if (p.M <= kFewMost && ik && jk && p.sum_batches == 1 && (p.K * size >= 2048 || tiles(64, 256) < 512)) {
         p.shape = kFewRows;
         return 0;
     }
     int64_t units = tiles(128, 128), full = 512;   // tiles, and how many are resident at once
-    if (!direct) {
+    if (units < 128 && p.M > 64 && p.N > 64) {
+        p.shape = kTileSmallAny;
+        units = tiles(64, 64), full = 768;
+    } else if (!direct) {
         p.shape = kTileMidAny;
     } else if (p.M <= 64) {
         p.shape = kTileLow;
@@ -325,9 +334,10 @@ int64_t ssmap::plan_product(Product &p, int dtype) {
     } else {
         p.shape = kTileMid;
     }
-    // Few tiles: the sum is split, in parts of eight stages at least (up to 128 tiles); with half of the tiles that
-    // fit at once only a long sum (2048 x 2048 from 8192 products, bf16: 112 -> 95 us; from 2048: 33 -> 42)
-    if (units && (units <= 128 ? steps >= 16 : units * 2 <= full && steps >= 96)) {
+    // Few tiles: the sum is split, in parts of eight stages at least; with half of the tiles that fit at once only
+    // a long sum.  2048 x 2048 results, bf16: from 8192 products 112 -> 95 us, from 2048 33 -> 42.  In small tiles
+    // 256 x 4096 from 4096 products 62 -> 37 us, 1024 x 1024 from 1024 16 -> 20.
+    if (units && (units <= 128 ? steps >= 16 : units * 2 <= full && steps >= (p.shape == kTileSmallAny ? 48 : 96))) {
         const int64_t most = steps / 8, want = full / units < most ? full / units : most;
         p.part_steps = (steps + want - 1) / want;
         p.splits = (int)((steps + p.part_steps - 1) / p.part_steps);

@@ -29,8 +29,13 @@ struct Product {
 };
 
 // Tile shapes (m x n).
-enum Shape { kTileBig = 0, kTileMid = 1, kTileLow = 2, kTileTall = 3, kTileMidAny = 4, kFewRows = 5 };
-constexpr int kFewMost = 32;                // rows kFewRows takes at most
+enum Shape { kTileBig = 0, kTileMid = 1, kTileLow = 2, kTileTall = 3, kTileMidAny = 4, kFewRows = 5, kHead = 6, kTileSmallAny = 7 };
+constexpr int kFewMost = 32;                // rows of a that kFewRows takes at most
+constexpr int kHeadMost = 64;               // rows of a that kHead takes at most, and their bytes in LDS
+constexpr int kHeadBytes = 64 << 10;
+// kHead's LDS rows: chunks, rounded up to whole swizzles of eight
+inline int64_t head_pitch(const Product &p, int size) { return (p.K * size / 16 + 7) / 8 * 8; }
+inline int64_t head_bytes(const Product &p, int size) { return (p.M + 15) / 16 * 16 * head_pitch(p, size) * 16; }
 
 inline unsigned blocks(int64_t n) { return (unsigned)(n < 1 ? 1 : n < (1 << 20) ? n : (1 << 20)); }
 
