@@ -25,43 +25,38 @@ inline bool direct_side(const void *p, int64_t line, int64_t out, int64_t sum, i
 constexpr int kDzRows = 128;       // rows: positions a block sums; 8 threads down, 32 packs of 8 outputs across
 constexpr int kDzPlane = 16384;    // planes: positions a block sums
 
-template <int DT, int OT>
-__device__ __forceinline__ void dz_pack(const elem_t<OT> *g, const elem_t<DT> *pre, elem_t<DT> *dz, int left, int act, float (&sum)[8]) {
-    float v[8] = {};
-    if (left >= 8) {
-        elem_t<OT> w[8];
-        __builtin_memcpy(w, g, sizeof w);
+// Eight neighbours, of which `left` exist; WHOLE: all, which the caller knows for its whole wave.
+template <bool WHOLE, int T>
+__device__ __forceinline__ void load8(const elem_t<T> *p, int left, float (&v)[8]) {
+    if constexpr (WHOLE) {
+        elem_t<T> w[8];
+        __builtin_memcpy(w, p, sizeof w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = Elem<OT>::get(w[e]);
+        for (int e = 0; e < 8; ++e) v[e] = Elem<T>::get(w[e]);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (e < left) v[e] = Elem<OT>::get(g[e]);
+        for (int e = 0; e < 8; ++e) v[e] = e < left ? Elem<T>::get(p[e]) : 0.0f;
     }
+}
+template <bool WHOLE, int DT, int OT>
+__device__ __forceinline__ void dz_pack(const elem_t<OT> *g, const elem_t<DT> *pre, elem_t<DT> *dz, int left, int act, float (&sum)[8]) {
+    float v[8];
+    load8<WHOLE, OT>(g, left, v);
     if (pre) {
-        float z[8] = {};
-        if (left >= 8) {
-            elem_t<DT> w[8];
-            __builtin_memcpy(w, pre, sizeof w);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) z[e] = Elem<DT>::get(w[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (e < left) z[e] = Elem<DT>::get(pre[e]);
-        }
+        float z[8];
+        load8<WHOLE, DT>(pre, left, z);
         with_activation(act, [&](auto a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] *= slope<a.value, DT == SSMAP_F32>(z[e]);
         });
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum[e] += v[e];
+    for (int e = 0; e < 8; ++e) sum[e] += WHOLE || e < left ? v[e] : 0.0f;
     if (dz) {
         elem_t<DT> w[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = Elem<DT>::put(v[e]);
-        if (left >= 8) {
+        if constexpr (WHOLE) {
             __builtin_memcpy(dz, w, sizeof w);
         } else {
 #pragma unroll
@@ -82,12 +77,16 @@ __global__ __launch_bounds__(256) void k_dz_rows(int64_t batch, int64_t rows, in
         const int64_t n = unit % strips * 256 + tx * 8, bc = unit / strips, b = bc / chunks, r0 = bc % chunks * kDzRows;
         const int left = (int)(outer - n < 8 ? outer - n : 8);
         float sum[8] = {};
-        if (left > 0)
-#pragma unroll 4
-            for (int64_t r = r0 + ty; r < (r0 + kDzRows < rows ? r0 + kDzRows : rows); r += 8) {
+        const int64_t end = r0 + kDzRows < rows ? r0 + kDzRows : rows;
+        const auto walk = [&](auto whole) {
+#pragma unroll 2
+            for (int64_t r = r0 + ty; r < end; r += 8) {
                 const int64_t o = (b * rows + r) * outer + n;
-                dz_pack<DT, OT>(g + b * g_batch + r * g_row + n, pre ? pre + o : nullptr, dz ? dz + o : nullptr, left, act, sum);
+                dz_pack<whole.value, DT, OT>(g + b * g_batch + r * g_row + n, pre ? pre + o : nullptr, dz ? dz + o : nullptr, left, act, sum);
             }
+        };
+        if (unit % strips * 256 + 256 <= outer) walk(std::true_type{});
+        else if (left > 0) walk(std::false_type{});
         if (!sums) continue;
         __syncthreads();
 #pragma unroll
@@ -111,10 +110,17 @@ __global__ __launch_bounds__(256) void k_dz_planes(int64_t batch, int64_t rows, 
         const int64_t c = unit % chunks, bn = unit / chunks, b = bn / outer, n = bn % outer;
         float sum[8] = {};
         const int64_t end = (c + 1) * kDzPlane < rows ? (c + 1) * kDzPlane : rows;
-        for (int64_t r = c * kDzPlane + threadIdx.x * 8; r < end; r += 2048) {
-            const int64_t o = bn * rows + r;
-            dz_pack<DT, OT>(g + b * g_batch + n * g_plane + r, pre ? pre + o : nullptr, dz ? dz + o : nullptr, (int)(end - r < 8 ? end - r : 8), act, sum);
+        const elem_t<OT> *gp = g + b * g_batch + n * g_plane;
+        const elem_t<DT> *zp = pre ? pre + bn * rows : nullptr;
+        elem_t<DT> *dp = dz ? dz + bn * rows : nullptr;
+        int64_t r = c * kDzPlane;
+#pragma unroll 2
+        for (; r + 2048 <= end; r += 2048) {
+            const int64_t at = r + threadIdx.x * 8;
+            dz_pack<true, DT, OT>(gp + at, zp ? zp + at : nullptr, dp ? dp + at : nullptr, 8, act, sum);
         }
+        const int64_t at = r + threadIdx.x * 8;
+        if (at < end) dz_pack<false, DT, OT>(gp + at, zp ? zp + at : nullptr, dp ? dp + at : nullptr, (int)(end - at < 8 ? end - at : 8), act, sum);
         if (!sums) continue;
         part[threadIdx.x] = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
         __syncthreads();

@@ -446,7 +446,7 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
                         store_run<true, SSMAP_F32, 8>(p.parts + split * p.out_batches * p.M * p.N, o, 8, z);
                     } else {
                         if (p.bias_along_m) load_bias<true, DT, 8>(p, m, n, 8, bias);
-                        finish<true, DT, OT, 8>(p, o, 8, z, bias, res);
+                        finish<true, DT, OT, 8, true>(p, o, 8, z, bias, res);
                     }
                     m += ROWS;
                     o += ROWS * p.N;
