@@ -39,7 +39,7 @@ __device__ __forceinline__ void load8(const elem_t<T> *p, int left, float (&v)[8
     }
 }
 template <bool WHOLE, int DT, int OT>
-__device__ __forceinline__ void dz_pack(const elem_t<OT> *g, const elem_t<DT> *pre, elem_t<DT> *dz, int left, int act, float (&sum)[8]) {
+__device__ __forceinline__ void dz_pack(const elem_t<OT> *g, const elem_t<DT> *pre, elem_t<DT> *dz, int left, int room, int act, float (&sum)[8]) {   // room: of dz's line, zeros included
     float v[8];
     load8<WHOLE, OT>(g, left, v);
     if (pre) {
@@ -61,7 +61,7 @@ __device__ __forceinline__ void dz_pack(const elem_t<OT> *g, const elem_t<DT> *p
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (e < left) dz[e] = w[e];
+                if (e < room) dz[e] = e < left ? w[e] : Elem<DT>::put(0.0f);
         }
     }
 }
@@ -69,7 +69,7 @@ __device__ __forceinline__ void dz_pack(const elem_t<OT> *g, const elem_t<DT> *p
 // sums[batch * row chunks][outer]
 template <int DT, int OT>
 __global__ __launch_bounds__(256) void k_dz_rows(int64_t batch, int64_t rows, int64_t outer, const elem_t<OT> *g, int64_t g_batch, int64_t g_row,
-                                                 const elem_t<DT> *pre, int act, elem_t<DT> *dz, float *sums) {
+                                                 const elem_t<DT> *pre, int act, elem_t<DT> *dz, int64_t dz_line, float *sums) {
     __shared__ float part[8][256];
     const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
     const int64_t strips = (outer + 255) / 256, chunks = (rows + kDzRows - 1) / kDzRows;
@@ -82,7 +82,7 @@ __global__ __launch_bounds__(256) void k_dz_rows(int64_t batch, int64_t rows, in
 #pragma unroll 2
             for (int64_t r = r0 + ty; r < end; r += 8) {
                 const int64_t o = (b * rows + r) * outer + n;
-                dz_pack<whole.value, DT, OT>(g + b * g_batch + r * g_row + n, pre ? pre + o : nullptr, dz ? dz + o : nullptr, left, act, sum);
+                dz_pack<whole.value, DT, OT>(g + b * g_batch + r * g_row + n, pre ? pre + o : nullptr, dz ? dz + (b * rows + r) * dz_line + n : nullptr, left, (int)(dz_line - n < 8 ? dz_line - n : 8), act, sum);
             }
         };
         if (unit % strips * 256 + 256 <= outer) walk(std::true_type{});
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256) void k_dz_rows(int64_t batch, int64_t rows, in
 // sums[batch * chunks][outer]
 template <int DT, int OT>
 __global__ __launch_bounds__(256) void k_dz_planes(int64_t batch, int64_t rows, int64_t outer, const elem_t<OT> *g, int64_t g_batch, int64_t g_plane,
-                                                   const elem_t<DT> *pre, int act, elem_t<DT> *dz, float *sums) {
+                                                   const elem_t<DT> *pre, int act, elem_t<DT> *dz, int64_t dz_line, float *sums) {
     __shared__ float part[256];
     const int64_t chunks = (rows + kDzPlane - 1) / kDzPlane;
     for (int64_t unit = blockIdx.x; unit < chunks * outer * batch; unit += gridDim.x) {
@@ -112,15 +112,16 @@ __global__ __launch_bounds__(256) void k_dz_planes(int64_t batch, int64_t rows, 
         const int64_t end = (c + 1) * kDzPlane < rows ? (c + 1) * kDzPlane : rows;
         const elem_t<OT> *gp = g + b * g_batch + n * g_plane;
         const elem_t<DT> *zp = pre ? pre + bn * rows : nullptr;
-        elem_t<DT> *dp = dz ? dz + bn * rows : nullptr;
+        elem_t<DT> *dp = dz ? dz + bn * dz_line : nullptr;
         int64_t r = c * kDzPlane;
 #pragma unroll 2
         for (; r + 2048 <= end; r += 2048) {
             const int64_t at = r + threadIdx.x * 8;
-            dz_pack<true, DT, OT>(gp + at, zp ? zp + at : nullptr, dp ? dp + at : nullptr, 8, act, sum);
+            dz_pack<true, DT, OT>(gp + at, zp ? zp + at : nullptr, dp ? dp + at : nullptr, 8, 8, act, sum);
         }
         const int64_t at = r + threadIdx.x * 8;
-        if (at < end) dz_pack<false, DT, OT>(gp + at, zp ? zp + at : nullptr, dp ? dp + at : nullptr, (int)(end - at < 8 ? end - at : 8), act, sum);
+        if (at < end) dz_pack<false, DT, OT>(gp + at, zp ? zp + at : nullptr, dp ? dp + at : nullptr, (int)(end - at < 8 ? end - at : 8),
+                                           (int)(end < rows ? 8 : dz_line - at < 8 ? dz_line - at : 8), act, sum);
         if (!sums) continue;
         part[threadIdx.x] = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
         __syncthreads();
@@ -183,7 +184,8 @@ int check_grad(const ssmap_linear_grad_args *a) {
 // The workspace of ssmap_linear_grad: dz, the bias's sums, the partial results of the products (one after
 // the other, so they share a place).
 struct GradPlan {
-    bool planes, copies;               // copies: dz differs from g
+    bool planes, copies;               // copies: dz is not g itself
+    int64_t dz_line;                   // values a line of dz takes: a multiple of 16 bytes, zeros behind the dense ones
     int64_t chunks;                    // sums a block leaves for each output
     Product x, w;
     int64_t dz_bytes, sum_bytes, part_bytes;
@@ -213,21 +215,26 @@ Product forward_product(const ssmap_linear_args *a) {
 GradPlan plan_grad(const ssmap_linear_grad_args *a) {
     GradPlan q{};
     q.planes = a->layout == SSMAP_PLANES;
-    q.copies = a->activation != SSMAP_ACT_NONE || a->grad_dtype != a->dtype;
+    const int size = head_dtype_size(a->dtype);
+    const int64_t e = 16 / size, dense = q.planes ? a->rows : a->outer;
+    // a dz of one's own also where g's lines are not at multiples of 16 bytes: both products read it
+    q.copies = a->activation != SSMAP_ACT_NONE || a->grad_dtype != a->dtype || reinterpret_cast<uintptr_t>(a->g) % 16 || a->g_inner_stride % e ||
+               a->g_batch_stride % e || dense % e;
+    q.dz_line = (dense + e - 1) / e * e;
     const int64_t chunk = q.planes ? kDzPlane : kDzRows;
     q.chunks = a->batch * ((a->rows + chunk - 1) / chunk);
-    q.dz_bytes = q.copies && (a->g_x || a->g_w) ? aligned(a->batch * a->rows * a->outer * head_dtype_size(a->dtype)) : 0;
+    q.dz_bytes = q.copies && (a->g_x || a->g_w) ? aligned(a->batch * (q.planes ? a->outer : a->rows) * q.dz_line * size) : 0;
     q.sum_bytes = a->g_bias ? aligned(q.chunks * a->outer * 4) : 0;
     // dz: [position][output] or [output][position] of a batch
     const void *dz = q.copies ? a->workspace : a->g;
-    const int64_t line = q.copies ? (q.planes ? a->rows : a->outer) : a->g_inner_stride, batch = q.copies ? a->rows * a->outer : a->g_batch_stride;
+    const int64_t line = q.copies ? q.dz_line : a->g_inner_stride, batch = q.copies ? (q.planes ? a->outer : a->rows) * q.dz_line : a->g_batch_stride;
     const int64_t to_row = q.planes ? 1 : line, to_out = q.planes ? line : 1;
-    Product &x = q.x;
+    Product &x = q.x, &w = q.w;
     x.M = a->rows; x.N = a->inner; x.K = a->outer; x.out_batches = a->batch; x.sum_batches = 1;
+    x.a_pads = w.a_pads = q.copies;
     x.a = dz; x.a_out = batch; x.a_m = to_row; x.a_k = to_out;
     x.b = a->w; x.b_n = 1; x.b_k = a->w_row_stride;
     x.out = a->g_x;
-    Product &w = q.w;
     w.M = a->outer; w.N = a->inner; w.K = a->rows; w.out_batches = 1; w.sum_batches = a->batch;
     w.a = dz; w.a_sum = batch; w.a_m = to_out; w.a_k = to_row;
     w.b = a->x; w.b_sum = a->x_batch_stride; w.b_n = 1; w.b_k = a->x_row_stride;
@@ -289,9 +296,9 @@ int ssmap_linear_grad(const ssmap_linear_grad_args *a, void *stream) {
         auto *dz = q.dz_bytes ? reinterpret_cast<elem_t<DT> *>(ws) : nullptr;
         if (positions * a->outer && (dz || sums)) {
             if (q.planes)
-                k_dz_planes<DT, OT><<<blocks(q.chunks * a->outer), 256, 0, st>>>(a->batch, a->rows, a->outer, g, a->g_batch_stride, a->g_inner_stride, pre, a->activation, dz, sums);
+                k_dz_planes<DT, OT><<<blocks(q.chunks * a->outer), 256, 0, st>>>(a->batch, a->rows, a->outer, g, a->g_batch_stride, a->g_inner_stride, pre, a->activation, dz, q.dz_line, sums);
             else
-                k_dz_rows<DT, OT><<<blocks(q.chunks * ((a->outer + 255) / 256)), 256, 0, st>>>(a->batch, a->rows, a->outer, g, a->g_batch_stride, a->g_inner_stride, pre, a->activation, dz, sums);
+                k_dz_rows<DT, OT><<<blocks(q.chunks * ((a->outer + 255) / 256)), 256, 0, st>>>(a->batch, a->rows, a->outer, g, a->g_batch_stride, a->g_inner_stride, pre, a->activation, dz, q.dz_line, sums);
         }
         if (a->g_bias && a->outer) k_bias_grad<DT><<<blocks((a->outer + 3) / 4), 256, 0, st>>>(q.chunks, a->outer, sums, static_cast<elem_t<DT> *>(a->g_bias));
         if (a->g_x) launch_product<DT, DT>(q.x, st);
@@ -306,10 +313,12 @@ int64_t ssmap::plan_product(Product &p, int dtype) {
     const int size = head_dtype_size(dtype);
     const bool ik = p.a_k == 1, jk = p.b_k == 1;
     p.splits = 1;
+    p.pack_a = p.pack_b = -1;
     const int64_t steps = (p.K * size + 127) / 128 * p.sum_batches;
     p.part_steps = steps;
-    const bool direct = direct_side(p.a, ik ? p.a_m : p.a_k, p.a_out, p.a_sum, ik ? p.K : p.M, size) &&
-                        direct_side(p.b, jk ? p.b_n : p.b_k, p.b_out, p.b_sum, jk ? p.K : p.N, size);
+    const bool direct_a = direct_side(p.a, ik ? p.a_m : p.a_k, p.a_out, p.a_sum, p.a_pads ? 0 : ik ? p.K : p.M, size);
+    const bool direct_b = direct_side(p.b, jk ? p.b_n : p.b_k, p.b_out, p.b_sum, jk ? p.K : p.N, size);
+    bool direct = direct_a && direct_b;
     const auto tiles = [&](int bi, int bj) { return (p.M + bi - 1) / bi * ((p.N + bj - 1) / bj) * p.out_batches; };
     const int64_t e = 16 / size;
     if (p.M <= kHeadMost && ik && jk && p.sum_batches == 1 && p.a_out == 0 && p.K >= e && p.K % e == 0 && head_bytes(p, size) <= kHeadBytes &&
@@ -322,8 +331,25 @@ int64_t ssmap::plan_product(Product &p, int dtype) {
         return 0;
     }
     int64_t units = tiles(128, 128), full = 512;   // tiles, and how many are resident at once
+    int64_t packed = 0;                            // bytes of the copies
+    if (!direct && p.M > 64 && p.N > 64 && (double)p.M * p.N * p.K * p.out_batches * p.sum_batches >= (dtype == SSMAP_F32 ? 1 << 28 : 1 << 30)) {
+        // Large enough to copy what is out of line first: 4097 x 4095 x 4099 bf16 takes 247 us with the copies and 361
+        // with loads through registers that straddle lines (gradient of x: 260 and 608); for less the launches cost
+        // more
+        const auto copy = [&](bool kc, int64_t rows, int64_t out) {
+            const int64_t lines = kc ? rows : p.K, dense = kc ? p.K : rows, at = packed;
+            packed += aligned((p.sum_batches > 1 ? p.sum_batches : out ? p.out_batches : 1) * lines * ((dense + e - 1) / e * e) * size);
+            return at;
+        };
+        // every line of a copy lies within 32-bit offsets of its tile
+        if (((ik ? p.K : p.M) + e) < (int64_t)1 << 21 && ((jk ? p.K : p.N) + e) < (int64_t)1 << 21) {
+            if (!direct_a) p.pack_a = copy(ik, p.M, p.a_out);
+            if (!direct_b) p.pack_b = copy(jk, p.N, p.b_out);
+            direct = true;
+        }
+    }
     if (units < 128 && p.M > 64 && p.N > 64) {
-        p.shape = kTileSmallAny;
+        p.shape = direct ? kTileSmall : kTileSmallAny;
         units = tiles(64, 64), full = 768;
     } else if (!direct) {
         p.shape = kTileMidAny;
@@ -343,10 +369,13 @@ int64_t ssmap::plan_product(Product &p, int dtype) {
     // Few tiles: the sum is split, in parts of eight stages at least; with half of the tiles that fit at once only
     // a long sum.  2048 x 2048 results, bf16: from 8192 products 112 -> 95 us, from 2048 33 -> 42.  In small tiles
     // 256 x 4096 from 4096 products 62 -> 37 us, 1024 x 1024 from 1024 16 -> 20.
-    if (units && (units <= 128 ? steps >= 16 : units * 2 <= full && steps >= (p.shape == kTileSmallAny ? 48 : 96))) {
+    if (units && (units <= 128 ? steps >= 16 : units * 2 <= full && steps >= (full > 512 ? 32 : 96))) {
         const int64_t most = steps / 8, want = full / units < most ? full / units : most;
         p.part_steps = (steps + want - 1) / want;
         p.splits = (int)((steps + p.part_steps - 1) / p.part_steps);
     }
-    return p.splits > 1 ? aligned(p.splits * p.out_batches * p.M * p.N * 4) : 0;
+    const int64_t parts = p.splits > 1 ? aligned(p.splits * p.out_batches * p.M * p.N * 4) : 0;
+    if (p.pack_a >= 0) p.pack_a += parts;
+    if (p.pack_b >= 0) p.pack_b += parts;
+    return parts + packed;
 }

@@ -26,10 +26,14 @@ struct Product {
     int64_t part_steps;
     int32_t splits, shape;                  // shape: see plan_product
     float *parts;
+    // operands whose lines do not start at multiples of 16 bytes are copied first, to lines that do: places
+    // behind `parts`, or -1
+    int64_t pack_a, pack_b;
+    bool a_pads;                            // a's lines are filled up with zeros to multiples of 16 bytes
 };
 
 // Tile shapes (m x n).
-enum Shape { kTileBig = 0, kTileMid = 1, kTileLow = 2, kTileTall = 3, kTileMidAny = 4, kFewRows = 5, kHead = 6, kTileSmallAny = 7 };
+enum Shape { kTileBig = 0, kTileMid = 1, kTileLow = 2, kTileTall = 3, kTileMidAny = 4, kFewRows = 5, kHead = 6, kTileSmallAny = 7, kTileSmall = 8 };
 constexpr int kFewMost = 32;                // rows of a that kFewRows takes at most
 constexpr int kHeadMost = 64;               // rows of a that kHead takes at most, and their bytes in LDS
 constexpr int kHeadBytes = 64 << 10;
@@ -39,7 +43,8 @@ inline int64_t head_bytes(const Product &p, int size) { return (p.M + 15) / 16 *
 
 inline unsigned blocks(int64_t n) { return (unsigned)(n < 1 ? 1 : n < (1 << 20) ? n : (1 << 20)); }
 
-// Chooses p.shape, p.splits and p.part_steps by sizes, strides and alignment; returns the bytes that p.parts needs.
+// Chooses p.shape, p.splits, p.part_steps and the copies by sizes, strides and alignment; returns the bytes that
+// p.parts needs.
 int64_t plan_product(Product &p, int dtype);
 // FINE: for results in float32.  Results of 16 bits take erfc from Abramowitz and Stegun's formula 7.1.26,
 // whose error of 1.5e-7 is far below their rounding.
@@ -99,6 +104,6 @@ __device__ __forceinline__ void with_activation(int act, F f) {
 
 // Enqueues a planned product of operands of type DT with results of type OT (DT or SSMAP_F32).
 template <int DT, int OT>
-void launch_product(const Product &p, hipStream_t st);
+void launch_product(Product p, hipStream_t st);
 
 }  // namespace ssmap

@@ -88,27 +88,36 @@ struct Side {
         }
     }
 
-    // Through registers, for any alignment and extent.
-    static __device__ __forceinline__ void load(i32x4 (&reg)[PER], const char *base, int rows, int ks, int64_t ld) {
+    // Through registers, for any alignment and extent.  Where everything exists (`all`, the same for the whole
+    // block) the loads have 32-bit offsets from one base and no branch between them.
+    static __device__ __forceinline__ void all_offsets(uint32_t (&off)[PER], uint32_t ld) {
+#pragma unroll
+        for (int it = 0; it < PER; ++it) {
+            int line, c;
+            place(it * NT + threadIdx.x, line, c);
+            off[it] = line * ld + c * 16;
+        }
+    }
+    static __device__ __forceinline__ void load(i32x4 (&reg)[PER], const char *base, const uint32_t (&off)[PER], bool all, int rows, int ks, int64_t ld) {
+        using loose = int __attribute__((ext_vector_type(4), aligned(2)));   // 16 bytes at any element
+        if (all) {
+#pragma unroll
+            for (int it = 0; it < PER; ++it) reg[it] = *reinterpret_cast<const loose *>(base + off[it]);
+            return;
+        }
 #pragma unroll
         for (int it = 0; it < PER; ++it) {
             int line, c;
             place(it * NT + threadIdx.x, line, c);
             const int n = count(line, c, rows, ks);
-            const char *p = base + line * ld + c * 16;
-            i32x4 v = {0, 0, 0, 0};
-            if (n == E) {
-                __builtin_memcpy(&v, p, 16);
-            } else {
-                elem_t<DT> e[E];
+            const elem_t<DT> *p = reinterpret_cast<const elem_t<DT> *>(base + line * ld + c * 16);
+            elem_t<DT> e[E];
 #pragma unroll
-                for (int q = 0; q < E; ++q) {
-                    e[q] = Elem<DT>::put(0.0f);
-                    if (q < n) e[q] = reinterpret_cast<const elem_t<DT> *>(p)[q];
-                }
-                __builtin_memcpy(&v, e, 16);
+            for (int q = 0; q < E; ++q) {
+                e[q] = Elem<DT>::put(0.0f);
+                if (q < n) e[q] = p[q];
             }
-            reg[it] = v;
+            __builtin_memcpy(&reg[it], e, 16);
         }
     }
     static __device__ __forceinline__ void store(const i32x4 (&reg)[PER], char *lds) {
@@ -285,7 +294,11 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
         if constexpr (DIRECT) {
             I::offsets(off_i, rows_i, I::KB, (uint32_t)ld_i);
             J::offsets(off_j, rows_j, I::KB, (uint32_t)ld_j);
+        } else {
+            I::all_offsets(off_i, (uint32_t)ld_i);
+            J::all_offsets(off_j, (uint32_t)ld_j);
         }
+        const bool all_i = rows_i == BI && ld_i < 1 << 24, all_j = rows_j == BJ && ld_j < 1 << 24;   // 256 lines: 32-bit offsets
         const auto fetch = [&](int buf) {   // stage `at` into buffer buf (DIRECT) or into registers
             const int64_t left = p.K - at * I::KB;
             const int ks = (int)(left < I::KB ? left : I::KB);
@@ -302,8 +315,8 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
                     J::fetch(pb, off_j, base + I::BYTES);
                 }
             } else {
-                I::load(reg_i, pa, rows_i, ks, ld_i);
-                J::load(reg_j, pb, rows_j, ks, ld_j);
+                I::load(reg_i, pa, off_i, all_i && ks == I::KB, rows_i, ks, ld_i);
+                J::load(reg_j, pb, off_j, all_j && ks == I::KB, rows_j, ks, ld_j);
             }
             advance();
         };
@@ -669,13 +682,59 @@ void launch_tiles(const Product &p, hipStream_t st) {
     if (p.shape == kTileMid) go(mid, mid, two, two, eight, two, std::true_type{});
     else if (p.shape == kTileLow) go(narrow, big, one, four, eight, two, std::true_type{});
     else if (p.shape == kTileTall) go(big, narrow, four, one, eight, two, std::true_type{});
+    else if (p.shape == kTileSmall) go(narrow, narrow, two, two, eight, four, std::true_type{});
     else if (p.shape == kTileSmallAny) go(narrow, narrow, two, two, eight, two, std::false_type{});
     else go(mid, mid, two, two, eight, two, std::false_type{});
 }
 
+// Lines of `dense` values to lines of `pitch` ones (a multiple of 16 bytes), filled up with zeros.
+template <int DT>
+__global__ __launch_bounds__(256) void k_pack(const elem_t<DT> *from, int64_t batch, int64_t line, int64_t batches, int64_t lines, int64_t dense,
+                                              int64_t pitch, elem_t<DT> *to) {
+    constexpr int E = 16 / sizeof(elem_t<DT>);
+    const int64_t chunks = pitch / E, units = batches * lines * chunks;
+    for (int64_t u = blockIdx.x * 256ll + threadIdx.x; u < units; u += gridDim.x * 256ll) {
+        const int64_t c = u % chunks, l = u / chunks % lines, b = u / chunks / lines;
+        const elem_t<DT> *src = from + b * batch + l * line + c * E;
+        i32x4 v;
+        if ((c + 1) * E <= dense) {
+            __builtin_memcpy(&v, src, 16);
+        } else {
+            elem_t<DT> e[E];
+#pragma unroll
+            for (int q = 0; q < E; ++q) {
+                e[q] = Elem<DT>::put(0.0f);
+                if (c * E + q < dense) e[q] = src[q];
+            }
+            __builtin_memcpy(&v, e, 16);
+        }
+        *reinterpret_cast<i32x4 *>(to + u * E) = v;
+    }
+}
+
+// Copies one operand (strides: dense across or along the sum) behind p.parts and points at the copy.
+template <int DT>
+void pack_side(const Product &p, int64_t at, bool kc, int64_t rows, const void *&side, int64_t &row, int64_t &k, int64_t &out, int64_t &sum, hipStream_t st) {
+    if (at < 0) return;
+    constexpr int64_t E = 16 / sizeof(elem_t<DT>);
+    const int64_t lines = kc ? rows : p.K, dense = kc ? p.K : rows, pitch = (dense + E - 1) / E * E;
+    const int64_t batches = p.sum_batches > 1 ? p.sum_batches : out ? p.out_batches : 1;
+    elem_t<DT> *to = reinterpret_cast<elem_t<DT> *>(reinterpret_cast<char *>(p.parts) + at);
+    const int64_t units = batches * lines * (pitch / E);
+    k_pack<DT><<<blocks((units + 255) / 256), 256, 0, st>>>(static_cast<const elem_t<DT> *>(side), p.sum_batches > 1 ? sum : out, kc ? row : k, batches, lines, dense,
+                                                            pitch, to);
+    side = to;
+    (kc ? row : k) = pitch;
+    if (out) out = lines * pitch;
+    if (p.sum_batches > 1) sum = lines * pitch;
+}
+
 template <int DT, int OT>
-void launch_product(const Product &p, hipStream_t st) {
+void launch_product(Product p, hipStream_t st) {
     if (p.M * p.N * p.out_batches == 0) return;
+    const bool ik = p.a_k == 1, jk = p.b_k == 1;
+    pack_side<DT>(p, p.pack_a, ik, p.M, p.a, p.a_m, p.a_k, p.a_out, p.a_sum, st);
+    pack_side<DT>(p, p.pack_b, jk, p.N, p.b, p.b_n, p.b_k, p.b_out, p.b_sum, st);
     if (p.shape == kFewRows) {
         const unsigned n = blocks((p.N + 15) / 16 * p.out_batches);
         if (p.M <= 16) k_few_rows<DT, OT, 1><<<n, kFewWaves * 64, 0, st>>>(p);
@@ -694,9 +753,9 @@ void launch_product(const Product &p, hipStream_t st) {
         else k_head<DT, OT, 4><<<n, 256, bytes, st>>>(p, pitch);
         return;
     }
-    if (p.a_k == 1 && p.b_k == 1) launch_tiles<DT, OT, true, true>(p, st);
+    if (ik && jk) launch_tiles<DT, OT, true, true>(p, st);
     else if constexpr (DT == OT) {
-        if (p.a_k == 1) launch_tiles<DT, OT, true, false>(p, st);
+        if (ik) launch_tiles<DT, OT, true, false>(p, st);
         else launch_tiles<DT, OT, false, false>(p, st);
     }
     if (p.splits > 1) {

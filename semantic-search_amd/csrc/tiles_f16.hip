@@ -5,7 +5,7 @@
 
 namespace ssmap {
 
-template void launch_product<SSMAP_F16, SSMAP_F16>(const Product &, hipStream_t);
-template void launch_product<SSMAP_F16, SSMAP_F32>(const Product &, hipStream_t);
+template void launch_product<SSMAP_F16, SSMAP_F16>(Product, hipStream_t);
+template void launch_product<SSMAP_F16, SSMAP_F32>(Product, hipStream_t);
 
 }  // namespace ssmap

@@ -5,6 +5,6 @@
 
 namespace ssmap {
 
-template void launch_product<SSMAP_F32, SSMAP_F32>(const Product &, hipStream_t);
+template void launch_product<SSMAP_F32, SSMAP_F32>(Product, hipStream_t);
 
 }  // namespace ssmap

@@ -473,7 +473,8 @@ def test_linear_planes(lead, K, N, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
-@pytest.mark.parametrize("n,K,N", [(8190, 200, 4088), (16400, 64, 2056), (4096, 1000, 8190), (40000, 128, 48), (2000, 2048, 1500), (100, 8200, 600)])
+@pytest.mark.parametrize("n,K,N", [(8190, 200, 4088), (16400, 64, 2056), (4096, 1000, 8190), (40000, 128, 48), (2000, 2048, 1500), (100, 8200, 600), (2047, 1001, 1037),
+                                   (1003, 515, 1501), (700, 1024, 520)])
 def test_linear_large(n, K, N, dtype):
     """Sizes that take the largest tiles, split sums and many tiles with partial ones at the ends; forward and
     backward against 64-bit products on the GPU."""
@@ -496,6 +497,31 @@ def test_linear_large(n, K, N, dtype):
     check("gradient of x", got.x, d @ wd, d.abs() @ wd.abs(), N)
     check("gradient of weight", got.weight, d.t() @ xd, d.abs().t() @ xd.abs(), n)
     check("gradient of bias", got.bias, d.sum(0), d.abs().sum(0), n)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("planes", [False, True])
+def test_linear_batches_out_of_line(planes, dtype):
+    """Batches that do not merge, rows that start anywhere, every size odd: copies of each batch are made."""
+    B, n, K, N = 3, 701, 1001, 603
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.full((B, n + 2, K + 4), math.nan, device="cuda", dtype=dtype)[:, 1:n + 1, 3:K + 3]
+    x.copy_(torch.randn((B, n, K), device="cuda", generator=g))
+    w = torch.full((N, K + 1), math.nan, device="cuda", dtype=dtype)[:, :K]
+    w.copy_(torch.randn((N, K), device="cuda", generator=g) / math.sqrt(K))
+    xd, wd = x.double(), w.double()
+    move = (lambda t: t.transpose(1, 2)) if planes else (lambda t: t)
+    check = lambda name, got, want, size, terms: close(name, got.double(), want.cpu(), (U * (terms + 8) * size * 1.0001 + HALF[dtype] * want.abs() * 1.0001 + SMALLEST[dtype]).cpu())  # noqa: E731
+    check("y", ssa.linear(x, w, planes=planes), move(xd @ wd.t()), move(xd.abs() @ wd.abs().t()), K)
+    dy = torch.full((B, N + 1, n + 1) if planes else (B, n + 1, N + 1), math.nan, device="cuda", dtype=dtype)
+    dy = dy[:, 1:, :n] if planes else dy[:, 1:, :N]
+    dy.copy_(torch.randn(dy.shape, device="cuda", generator=g))
+    got = ssa.linear_grad(dy, x, w, planes=planes)
+    d = move(dy.double())
+    check("gradient of x", got.x, d @ wd, d.abs() @ wd.abs(), N)
+    df, xf = d.reshape(-1, N), xd.reshape(-1, K)
+    check("gradient of weight", got.weight, df.t() @ xf, df.abs().t() @ xf.abs(), B * n)
+    check("gradient of bias", got.bias, df.sum(0), df.abs().sum(0), B * n)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
