@@ -333,7 +333,7 @@ int ssmap_log_probs(const ssmap_log_probs_args *args, void *stream);
  *   d / d logit_j = ( g_l ([j = id] - p_j) + sum_k g_top_k ([j = top_id_k] - p_j)
  *                     - g_e p_j (log p_j + entropy) ) / temperature.
  * row_max, log_sum, entropy and top_ids are ssmap_log_probs' answers for the same logits.  Ignored ids
- * and alternatives of id -1 give nothing.  A position whose classes are all masked has the gradient 0;
+ * and alternatives with an id outside [0, classes) give nothing; no alternative stands twice in a position.  A position whose classes are all masked has the gradient 0;
  * one without a distribution, or with an id outside [0, classes) and a g_log_prob given, NaN.  A
  * gradient that is NULL counts as 0. */
 typedef struct ssmap_log_probs_grad_args {

@@ -643,7 +643,10 @@ __global__ __launch_bounds__(kThreads) void k_grad_rows(Shape s, const elem_t<DT
         const bool bad = log_sum != log_sum || (given && !inside);
         const int top = g.g_top && !none ? s.top : 0;
         float gl = given ? g.g_log_prob[pos] : 0.0f, all = gl;
-        for (int k = 0; k < top; ++k) all += g.top_ids[pos * s.top + k] >= 0 ? g.g_top[pos * s.top + k] : 0.0f;
+        for (int k = 0; k < top; ++k) {
+            const int32_t c = g.top_ids[pos * s.top + k];
+            all += c >= 0 && c < s.classes ? g.g_top[pos * s.top + k] : 0.0f;
+        }
         const float ge = g.g_entropy ? g.g_entropy[pos] : 0.0f, h = g.g_entropy ? g.entropy[pos] : 0.0f;
         float A = -(all + ge * h) * s.inv_t, B = -ge * kLn2 * s.inv_t;
         gl *= s.inv_t;
@@ -676,7 +679,7 @@ __global__ __launch_bounds__(kThreads) void k_grad_rows(Shape s, const elem_t<DT
             bool waited = false;
             for (int k = sub; k < top; k += LPR) {
                 const int64_t c = g.top_ids[pos * s.top + k];
-                if (c < c0 || c >= c0 + LPR * VEC * U) continue;
+                if (c < c0 || c >= c0 + LPR * VEC * U || c >= s.classes) continue;
                 if (!waited) {   // the stores above come from other lanes of this wave
                     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                     waited = true;
@@ -719,6 +722,7 @@ __global__ __launch_bounds__(kThreads) void k_grad_planes(Shape s, const elem_t<
             const int64_t tat = (b * s.top + k) * s.rows + r;
             const bool on = tops && k < s.top;
             ti[q][k] = on ? g.top_ids[tat] : -1;
+            if (ti[q][k] >= s.classes) ti[q][k] = -1;
             gt[q][k] = on && ti[q][k] >= 0 ? g.g_top[tat] : 0.0f;
             all += gt[q][k];
         }

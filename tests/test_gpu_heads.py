@@ -357,6 +357,23 @@ def test_grad_takes_expanded_gradients_and_views():
     check_grad(got.view(-1, 51), flat, fid, 1.0, plain_scores(flat, fid, 1.0, 2), torch.full((21,), -0.25), None, None)
 
 
+def test_grad_leaves_alternatives_outside_alone():
+    """Ids of alternatives that no class has give nothing, and nothing is written behind a row."""
+    for V, planes in ((700, False), (40, False), (5000, False), (40, True)):
+        x, ids = make_rows(4, V, torch.float32, V)
+        dx = (x.t()[None].contiguous() if planes else x).cuda()
+        t = (ids[None] if planes else ids).cuda()
+        d = 1 if planes else -1
+        s = ssa.log_probs(dx, t, dim=d, top=3)
+        g_t = torch.ones_like(s.top_log_prob)
+        bad = s.top_ids.clone()
+        bad.select(d, 1).copy_(torch.tensor([V, V + 1, 2 ** 31 - 1, -7])[None] if planes else torch.tensor([V, V + 1, 2 ** 31 - 1, -7]))
+        got = ssa.log_probs_grad(dx, t, s._replace(top_ids=bad), dim=d, grad_top=g_t)
+        none = s.top_ids.clone()
+        none.select(d, 1).fill_(-1)
+        assert torch.equal(got, ssa.log_probs_grad(dx, t, s._replace(top_ids=none), dim=d, grad_top=g_t))
+
+
 def test_grad_against_differences():
     """Central differences of the 64-bit forward formula, step 1e-4: its own error is below 1e-7."""
     x, ids = make_rows(2, 9, torch.float32, 1)
