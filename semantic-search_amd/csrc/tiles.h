@@ -8,6 +8,10 @@
 // is turned while it is read: ds_read_b64_tr_b16 gives lane q of 16 the values of column q from four rows of
 // 16 columns.  Its chunks are swizzled by 32 bytes a row, so that the four rows lie in different banks.
 //
+// What bounds it at large sizes is the way from L2 to LDS: at 8192^3 bf16 the loads alone take 711 us, the matrix
+// instructions alone 674, both together 890 to 925 (1190 to 1240 TFLOP/s).  So tiles are as large as the registers
+// hold, and the turns below keep the loads from holding up the reads.
+//
 // The matrix instruction takes J as its rows and I as its columns: a lane then holds four neighbouring n of
 // one m, which the epilogue reads and writes together.
 #pragma once
@@ -526,7 +530,8 @@ __global__ __launch_bounds__(256) void k_join_parts(Product p) {
 
 // At most 16 MT rows of a (single tokens, small batches) against all of b: reading b once is all the work.  A
 // block takes 16 rows of b, its eight waves share the sum; both operands go from memory to registers as the
-// matrix instruction wants them, eight loads of b under way in each wave.
+// matrix instruction wants them, eight loads of b under way in each wave.  3 x 4096 x 4096 bf16 takes 9.5 us, 3.5
+// TB/s; a 64 x 256 tile with a split sum 20.
 constexpr int kFewWaves = 8;
 template <int DT, int OT, int MT>
 __global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(Product p) {
