@@ -164,6 +164,7 @@ int check(const Args *a, int other) {
     if (a->layout != SSMAP_ROWS && a->layout != SSMAP_PLANES)
         return head_error(SSMAP_ERR_INVALID_ARG, "layout is neither SSMAP_ROWS nor SSMAP_PLANES");
     if (a->activation < SSMAP_ACT_NONE || a->activation > SSMAP_ACT_SILU) return head_error(SSMAP_ERR_INVALID_ARG, "unknown activation");
+    if (a->x_batch_stride < 0 || a->x_row_stride < 0 || a->w_row_stride < 0) return head_error(SSMAP_ERR_INVALID_ARG, "strides must not be negative");
     if (!head_sizes_ok(a->batch, a->rows, a->inner) || !head_sizes_ok(a->batch, a->rows, a->outer) || !head_sizes_ok(1, a->outer, a->inner))
         return head_error(SSMAP_ERR_INVALID_ARG, "sizes must not be negative, and no tensor may have 2^40 elements");
     return SSMAP_OK;
@@ -174,11 +175,13 @@ int check_linear(const ssmap_linear_args *a) {
     if (int rc = check(a, a->out_dtype)) return rc;
     if (a->bias && a->bias_dtype != a->dtype && a->bias_dtype != SSMAP_F32)
         return head_error(SSMAP_ERR_INVALID_ARG, "the bias's type must be dtype or SSMAP_F32");
+    if (a->res_batch_stride < 0 || a->res_inner_stride < 0) return head_error(SSMAP_ERR_INVALID_ARG, "strides must not be negative");
     return SSMAP_OK;
 }
 
 int check_grad(const ssmap_linear_grad_args *a) {
     if (!a) return head_error(SSMAP_ERR_INVALID_ARG, "null argument");
+    if (a->g_batch_stride < 0 || a->g_inner_stride < 0) return head_error(SSMAP_ERR_INVALID_ARG, "strides must not be negative");
     return check(a, a->grad_dtype);
 }
 

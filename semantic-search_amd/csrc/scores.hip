@@ -788,6 +788,8 @@ int check(const Args *a, Shape &s) {
         return head_error(SSMAP_ERR_INVALID_ARG, "top must be in [0, min(32, classes)]");
     if (!(a->temperature >= 1e-30f && a->temperature <= 1e30f))
         return head_error(SSMAP_ERR_INVALID_ARG, "temperature must be in [1e-30, 1e30]");
+    if (a->batch_stride < 0 || a->inner_stride < 0 || a->ids_batch_stride < 0 || a->ids_row_stride < 0)
+        return head_error(SSMAP_ERR_INVALID_ARG, "strides must not be negative");
     s.batch = a->batch; s.rows = a->rows; s.classes = a->classes;
     s.batch_stride = a->batch_stride;
     s.class_stride = a->layout == SSMAP_ROWS ? 1 : a->inner_stride;
@@ -890,7 +892,8 @@ int ssmap_log_probs(const ssmap_log_probs_args *a, void *stream) {
     if (!a->logits || !a->ids || !a->log_prob || !a->entropy || !a->row_max || !a->log_sum || (a->top && (!a->top_ids || !a->top_log_prob)))
         return head_error(SSMAP_ERR_INVALID_ARG, "null argument");
     const int64_t need = ssmap_log_probs_workspace(a);
-    if (a->workspace_bytes < need || (need && !a->workspace)) return head_error(SSMAP_ERR_INVALID_ARG, "the workspace is smaller than ssmap_log_probs_workspace says");
+    if (a->workspace_bytes < need || (need && (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 16)))
+        return head_error(SSMAP_ERR_INVALID_ARG, "the workspace is not at a multiple of 16 or smaller than ssmap_log_probs_workspace says");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (a->dtype == SSMAP_F32) launch_scores<SSMAP_F32>(s, *a, st);
     else if (a->dtype == SSMAP_BF16) launch_scores<SSMAP_BF16>(s, *a, st);

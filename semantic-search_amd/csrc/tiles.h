@@ -85,10 +85,12 @@ struct Side {
         const uint32_t first = lds + (threadIdx.x / 64) * 1024;
 #pragma unroll
         for (int it = 0; it < PER; ++it) {
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
+            // Five wait states: the descriptor may come out of vector lanes (a spilled scalar register), and the
+            // compiler counts none of its own in front of an instruction it does not see.
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(
                              __builtin_amdgcn_readfirstlane(first + it * NT * 16)),
                          "v"(off[it]), "s"(desc)
-                         : "memory");
+                         : "memory");   // m0 is reserved: the compiler keeps nothing in it
         }
     }
 

@@ -336,7 +336,7 @@ class MapEngine:
             raise ValueError(f"weight: expected [{self.n_classes}, D] on {self.device}, got {tuple(weight.shape)} on {weight.device}")
         if bias is not None and tuple(bias.shape) != (self.n_classes,):
             raise ValueError(f"bias: expected ({self.n_classes},), got {tuple(bias.shape)}")
-        self._head = (weight, bias)
+        self._head = (weight.detach(), None if bias is None else bias.detach())
 
     def head_logits(self, features: torch.Tensor) -> torch.Tensor:
         """float32 class planes [E, C, H, W] = features [E, H, W, D] times the head, for `step` and `stage1`."""
@@ -346,7 +346,8 @@ class MapEngine:
         shape = (self.n_envs, self.img_h, self.img_w, weight.shape[1])
         if tuple(features.shape) != shape:
             raise ValueError(f"features: expected {shape}, got {tuple(features.shape)}")
-        return heads.linear(features, weight, bias, planes=True, out_dtype=torch.float32)
+        with torch.no_grad():   # the maps carry no gradient
+            return heads.linear(features, weight, bias, planes=True, out_dtype=torch.float32)
 
     # ---- one batch of frames
     def step(self, depth: torch.Tensor, agent_pose, camera_pose, goal_sem_ids, *,

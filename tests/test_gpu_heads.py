@@ -517,6 +517,29 @@ def test_linear_large(n, K, N, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("K,N", [(8, 1), (24, 17), (72, 40), (256, 40), (512, 64), (2048, 16), (40, 33)])
+def test_linear_heads(K, N, dtype):
+    """Few classes against many positions, in planes of several frames that start anywhere, and few rows against
+    a vocabulary; NaN beside what may be read."""
+    B, n = 2, 9001
+    g = torch.Generator(device="cuda").manual_seed(K)
+    x = torch.full((B, n + 1, K + 3), math.nan, device="cuda", dtype=dtype)[:, :n, 1:K + 1]
+    x.copy_(torch.randn((B, n, K), device="cuda", generator=g))
+    w = torch.full((N + 1, K + 5), math.nan, device="cuda", dtype=dtype)[:N, 3:K + 3]
+    w.copy_(torch.randn((N, K), device="cuda", generator=g) / math.sqrt(K))
+    b = torch.randn(N, device="cuda", generator=g)
+    r = torch.randn((B, N, n), device="cuda", generator=g)
+    ref, _, size = plain_linear(x, w, b, "silu", r, True)
+    got = ssa.linear(x, w, b, activation="silu", residual=r, planes=True, out_dtype=torch.float32)
+    close("planes", got, ref.cpu(), linear_tolerance(ref, ref - r.double(), size, K, torch.float32).cpu())
+    tokens, vocab = w[:min(N, 40)], x[0].reshape(n, K).repeat(2, 1)
+    bias = torch.randn(vocab.shape[0], device="cuda", generator=g)
+    ref, _, size = plain_linear(tokens, vocab, bias, None, None, False)
+    got = ssa.linear(tokens, vocab, bias)
+    close("rows", got, ref.cpu(), linear_tolerance(ref, ref, size, K, dtype).cpu())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
 @pytest.mark.parametrize("planes", [False, True])
 def test_linear_batches_out_of_line(planes, dtype):
     """Batches that do not merge, rows that start anywhere, every size odd: copies of each batch are made."""
@@ -707,7 +730,7 @@ def test_engine_step_from_features(dtype):
         engines.append(eng)
     with pytest.raises(RuntimeError, match="set_head"):
         engines[0].head_logits(torch.zeros((E, h, w_, D), dtype=dtype, device="cuda"))
-    engines[0].set_head(weight, bias)
+    engines[0].set_head(torch.nn.Parameter(weight), bias)      # a module's own weight: the engine records nothing
     rng = np.random.default_rng(0)
     for i in range(2):
         frames = []

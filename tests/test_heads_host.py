@@ -109,6 +109,13 @@ def _args(kind, **over):
     ("log_probs", dict(temperature=float("nan")), "temperature must be"),
     ("log_probs", dict(temperature=float("inf")), "temperature must be"),
     ("log_probs", dict(temperature=-1.0), "temperature must be"),
+    ("log_probs", dict(inner_stride=-1), "strides"),
+    ("log_probs_grad", dict(ids_row_stride=-1), "strides"),
+    ("linear", dict(x_row_stride=-3), "strides"),
+    ("linear", dict(res_inner_stride=-3), "strides"),
+    ("linear_grad", dict(g_inner_stride=-3), "strides"),
+    ("log_probs", dict(rows=2, classes=1 << 20, workspace=1 << 20 | 4, workspace_bytes=1 << 30), "multiple of 16"),
+    ("linear_grad", dict(workspace=1 << 20 | 4), "multiple of 16"),
     ("log_probs", dict(logits=None), "null"),
     ("log_probs", dict(entropy=None), "null"),
     ("log_probs", dict(top=1, top_ids=None), "null"),
