@@ -352,31 +352,52 @@ int64_t ssmap::plan_product(Product &p, int dtype) {
             direct = true;
         }
     }
-    if (units < 128 && p.M > 64 && p.N > 64) {
-        p.shape = direct ? kTileSmall : kTileSmallAny;
-        units = tiles(64, 64), full = 768;
-    } else if (!direct) {
-        p.shape = kTileMidAny;
-    } else if (p.M <= 64) {
-        p.shape = kTileLow;
-        units = tiles(64, 256);
-    } else if (p.N <= 64) {
-        p.shape = kTileTall;
-        units = tiles(256, 64);
-    } else if (dtype != SSMAP_F32 && tiles(256, 256) >= 192) {
-        // three quarters of a round of the large tile and more: 112 against 127 us at 4096^3 bf16 (256 tiles)
-        p.shape = kTileBig;
-        units = tiles(256, 256), full = 256;
+    if (dtype == SSMAP_F32 && direct) {
+        // float32 matrix instructions take sixteen times as long, so how evenly the tiles fill the CUs decides: the
+        // shape and split whose busiest CU is done first, with a stage of a 128 x 128 tile (or its like) at 2.1 us, of a
+        // 64 x 64 tile at 0.8 us, and a join at 4 us and its bytes at 4 TB/s (all measured)
+        double best = 1e30;
+        const auto consider = [&](int shape, int64_t tiles_n, double stage) {
+            for (int64_t s = 1; s <= 512 && (s == 1 || steps / s >= 4); s = s < 16 ? s + 1 : s * 2) {
+                const int64_t part = (steps + s - 1) / s, n = (steps + part - 1) / part;
+                const double us = (double)((tiles_n * n + 255) / 256) * part * stage + (n > 1 ? 4.0 + 8e-6 * n * p.out_batches * p.M * p.N / 4 : 0.0);
+                if (us < best) best = us, p.shape = shape, p.part_steps = part, p.splits = (int)n;
+            }
+        };
+        if (steps == 0) p.shape = kTileMid;
+        else if (p.M <= 64) consider(kTileLow, tiles(64, 256), 2.1);
+        else if (p.N <= 64) consider(kTileTall, tiles(256, 64), 2.1);
+        else {
+            consider(kTileMid, tiles(128, 128), 2.1);
+            consider(kTileSmall, tiles(64, 64), 0.8);
+        }
     } else {
-        p.shape = kTileMid;
-    }
-    // Few tiles: the sum is split, in parts of eight stages at least; with half of the tiles that fit at once only
-    // a long sum.  2048 x 2048 results, bf16: from 8192 products 112 -> 95 us, from 2048 33 -> 42.  In small tiles
-    // 256 x 4096 from 4096 products 62 -> 37 us, 1024 x 1024 from 1024 16 -> 20.
-    if (units && (units <= 128 ? steps >= 16 : units * 2 <= full && steps >= (full > 512 ? 32 : 96))) {
-        const int64_t most = steps / 8, want = full / units < most ? full / units : most;
-        p.part_steps = (steps + want - 1) / want;
-        p.splits = (int)((steps + p.part_steps - 1) / p.part_steps);
+        if (units < 128 && p.M > 64 && p.N > 64) {
+            p.shape = direct ? kTileSmall : kTileSmallAny;
+            units = tiles(64, 64), full = 768;
+        } else if (!direct) {
+            p.shape = kTileMidAny;
+        } else if (p.M <= 64) {
+            p.shape = kTileLow;
+            units = tiles(64, 256);
+        } else if (p.N <= 64) {
+            p.shape = kTileTall;
+            units = tiles(256, 64);
+        } else if (dtype != SSMAP_F32 && tiles(256, 256) >= 192) {
+            // three quarters of a round of the large tile and more: 112 against 127 us at 4096^3 bf16 (256 tiles)
+            p.shape = kTileBig;
+            units = tiles(256, 256), full = 256;
+        } else {
+            p.shape = kTileMid;
+        }
+        // Few tiles: the sum is split, in parts of eight stages at least; with half of the tiles that fit at once only
+        // a long sum.  2048 x 2048 results, bf16: from 8192 products 112 -> 95 us, from 2048 33 -> 42.  In small tiles
+        // 256 x 4096 from 4096 products 62 -> 37 us, 1024 x 1024 from 1024 16 -> 20.
+        if (units && (units <= 128 ? steps >= 16 : units * 2 <= full && steps >= (full > 512 ? 32 : 96))) {
+            const int64_t most = steps / 8, want = full / units < most ? full / units : most;
+            p.part_steps = (steps + want - 1) / want;
+            p.splits = (int)((steps + p.part_steps - 1) / p.part_steps);
+        }
     }
     const int64_t parts = p.splits > 1 ? aligned(p.splits * p.out_batches * p.M * p.N * 4) : 0;
     if (p.pack_a >= 0) p.pack_a += parts;
