@@ -278,7 +278,7 @@ int ssmap_path_paint(ssmap_engine *eng, void *stream);
  *
  * They belong to no engine: the caller passes device pointers, shapes and strides (in elements), a
  * stream of the current device and, where ssmap_*_workspace() asks for one, a workspace that is used by
- * this call alone until its work on the stream is done.  Nothing is allocated, nothing waits, nothing is
+ * this call alone until its work on the stream is done (at a multiple of 16 bytes).  Strides are not negative.  Nothing is allocated, nothing waits, nothing is
  * kept between calls, so a call may be captured into a graph and replayed.  No counterpart in the
  * reference, whose networks end in library calls (infer.py:95-118, 301-327 hold what follows them).
  *
@@ -377,7 +377,7 @@ typedef struct ssmap_linear_args {
     void *workspace;
     int64_t workspace_bytes;
 } ssmap_linear_args;
-int64_t ssmap_linear_workspace(const ssmap_linear_args *args);
+int64_t ssmap_linear_workspace(const ssmap_linear_args *args);   /* bytes; strides and the pointers' alignment count; -1: refused */
 int ssmap_linear(const ssmap_linear_args *args, void *stream);
 
 /* The gradients of ssmap_linear from g = dL/dy.  With dz = g act'(pre):
@@ -400,7 +400,7 @@ typedef struct ssmap_linear_grad_args {
     void *workspace;
     int64_t workspace_bytes;
 } ssmap_linear_grad_args;
-int64_t ssmap_linear_grad_workspace(const ssmap_linear_grad_args *args);
+int64_t ssmap_linear_grad_workspace(const ssmap_linear_grad_args *args);   /* as above; which outputs are NULL counts too */
 int ssmap_linear_grad(const ssmap_linear_grad_args *args, void *stream);
 
 const char *ssmap_last_error(void);

@@ -245,6 +245,32 @@ def test_views(V, dtype):
         assert torch.equal(a, b)
 
 
+def test_offsets_past_31_bits():
+    """The last rows of tensors of more than 2^31 elements, against the same rows by themselves."""
+    n, V = 16400, 131072
+    x = torch.zeros((n, V), dtype=torch.bfloat16, device="cuda")
+    x[-3:] = torch.randn((3, V), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) * 3
+    ids = torch.arange(n, device="cuda") % V
+    s = ssa.log_probs(x, ids, top=5)
+    want = plain_scores(x[-3:].cpu(), ids[-3:].cpu(), 1.0, 5)
+    check_scores(ssa.LogProbs(*[t[-3:] for t in s]), want, V)
+    g_l, g_e = torch.ones(n, device="cuda"), torch.full((n,), 0.5, device="cuda")
+    g = ssa.log_probs_grad(x, ids, s, grad_log_prob=g_l, grad_entropy=g_e)
+    check_grad(g[-3:], x[-3:].cpu(), ids[-3:].cpu(), 1.0, want, g_l[-3:].cpu(), g_e[-3:].cpu(), None)
+    del g
+    w = torch.randn((16, V), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).bfloat16()
+    y = ssa.linear(x, w, out_dtype=torch.float32)
+    ref = x[-3:].double() @ w.double().t()
+    close("y", y[-3:], ref.cpu(), (U * (V + 8) * (x[-3:].double().abs() @ w.double().abs().t())).cpu())
+    planes = torch.zeros((1, 8, 270_000_000), dtype=torch.bfloat16, device="cuda")
+    planes[0, :, -5:] = torch.randn((8, 5), device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    t = torch.full((1, 270_000_000), 3, dtype=torch.int32, device="cuda")
+    s = ssa.log_probs(planes, t, dim=1)
+    rows = planes[0, :, -5:].t().cpu()
+    check_scores(ssa.LogProbs(*[v[0, ..., -5:] if v.numel() else v.view(0).new_zeros((5, 0)) for v in s]),
+                 plain_scores(rows, torch.full((5,), 3), 1.0, 0), 8)
+
+
 def test_empty_and_one_dimensional():
     got = ssa.log_probs(torch.zeros(0, 9, device="cuda"), torch.zeros(0, dtype=torch.int64, device="cuda"), top=2)
     assert got.log_prob.shape == (0,) and got.top_ids.shape == (0, 2)
