@@ -162,8 +162,7 @@ struct Side {
 };
 
 // N values next to each other, of which `left` exist; WHOLE: all of them, which the caller knows for its whole
-// wave (with a branch for each lane the compiler merges both ways into pieces: 1108 against 1359 us at 8192^3
-// in 128 wide tiles).
+// wave (with a branch for each lane the compiler merges both ways into pieces of 2 to 12 bytes).
 template <int DT, int N>
 struct Run {
     elem_t<DT> v[N];
@@ -334,14 +333,14 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
         };
         f32x4 acc[TI][TJ] = {};
         i32x4 fi[TI], fj[TJ];
-        const auto read = [&](int buf, int kk) {
+        const auto read = [&](int buf, int kk, i32x4 (&fi)[TI], i32x4 (&fj)[TJ]) {
             const char *li = stage(buf), *lj = li + I::BYTES;
 #pragma unroll
             for (int i = 0; i < TI; ++i) fi[i] = I::read(li, (wi * TI + i) * 16, kk);
 #pragma unroll
             for (int j = 0; j < TJ; ++j) fj[j] = J::read(lj, (wj * TJ + j) * 16, kk);
         };
-        const auto multiply = [&] {
+        const auto multiply = [&](const i32x4 (&fi)[TI], const i32x4 (&fj)[TJ]) {
 #pragma unroll
             for (int i = 0; i < TI; ++i)
 #pragma unroll
@@ -354,7 +353,7 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
             // turns 4t and 4t + 2 and multiply them in the turns behind; the second waves read the last half of
             // stage t - 1 in turn 4t - 1.  So from turn 4t on that stage's buffer is free for stage t + 1: the
             // first waves send for it in turn 4t, the second ones in turn 4t + 1, each behind its reads (in front
-            // of them or of the matrix instructions the queue of loads held those up: 978 against 922 us at
+            // of them or of the matrix instructions the queue of loads held those up: 937 against 896 us at
             // 8192^3), and all have waited for it at the end of turn 4t + 3.
             static_assert(DIRECT && C == 8 && NBUF == 2, "two turns a stage");
             const bool late = wave >= 4;
@@ -373,21 +372,21 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
                 if (late) turn_ends();
                 for (int64_t t = first; t < last; ++t) {
                     const int buf = (int)((t - first) & 1);
-                    read(buf, 0);
+                    read(buf, 0, fi, fj);
                     __builtin_amdgcn_sched_barrier(0);
                     if (t + 1 < last) fetch(buf ^ 1);
                     have_read();
                     turn_ends();
                     __builtin_amdgcn_s_setprio(1);
-                    multiply();
+                    multiply(fi, fj);
                     __builtin_amdgcn_s_setprio(0);
                     turn_ends();
-                    read(buf, 1);
+                    read(buf, 1, fi, fj);
                     if (late) have_landed();
                     have_read();
                     turn_ends();
                     __builtin_amdgcn_s_setprio(1);
-                    multiply();
+                    multiply(fi, fj);
                     __builtin_amdgcn_s_setprio(0);
                     if (!late) have_landed();
                     turn_ends();
@@ -417,20 +416,25 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
                 const int next = buf ? buf - 1 : NBUF - 1;
                 const bool more = sent < last;
                 if (more) fetch(next), ++sent;
-#pragma unroll
-                for (int kk = 0; kk < C / 4; ++kk) {
-                    read(buf, kk);
-                    multiply();
-                }
+                // Both halves' operands first, in registers of their own: left to itself the compiler reads each into
+                // the same few registers in front of the matrix instructions that want it, and waits every time
+                // (8192 x 4096 x 8192 bf16 in 128 wide tiles: 643 against 601 us).  The loads are sent in front of
+                // the reads here: two blocks a CU keep each other busy, and behind the reads they come late (626).
+                i32x4 gi[TI], gj[TJ];
+                read(buf, 0, fi, fj);
+                if constexpr (C == 8) read(buf, 1, gi, gj);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(fi, fj);
+                if constexpr (C == 8) multiply(gi, gj);
                 if (more) keep(next);
                 buf = buf + 1 == NBUF ? 0 : buf + 1;
             }
         }
         __syncthreads();   // nobody reads the stages any more
         // Each wave turns its own results round in LDS, HI rows of 16 at a time: out of the registers with four
-        // neighbouring n a lane, back with eight.  Loops stay loops here: the code runs once a tile, and
-        // unrolled it costs more in instruction fetches than the whole epilogue (112 of 537 us at 8192 x 4096 x
-        // 8192).  The residual of the next rows is under way while these are finished.
+        // neighbouring n a lane, back with eight.  Loops stay loops here: the code runs once a tile and
+        // is fetched anew each time (8192 x 4096 x 8192 bf16 with gelu and residual: 536 us unrolled, 502 so).  The
+        // residual of the next rows is under way while these are finished.
         const int lane = threadIdx.x % 64, q = lane % 16, g = lane / 16;
         float *turn = reinterpret_cast<float *>(lds_all + wave * (HI * 16 * PITCH * 4));
         const int col = lane % LINE * 8;
