@@ -382,8 +382,10 @@ int ssmap_linear(const ssmap_linear_args *args, void *stream);
 
 /* The gradients of ssmap_linear from g = dL/dy.  With dz = g act'(pre):
  *   g_x = dz w,   g_w = dz^T x,   g_bias = sum of dz over the positions   (g itself is the residual's).
- * dz is rounded to dtype before the two products (their operands are the matrix instructions' types) and
- * summed unrounded for g_bias.  Outputs that are NULL are left out. */
+ * Where dtype has 16 bits and g is float32 or an activation is given, dz goes into the two products as two values of
+ * dtype, the rounded one and what the rounding left (the matrix instructions' operands have no more bits): 16 bits of
+ * it for SSMAP_BF16, 22 for SSMAP_F16.  An infinite x or w then can make NaN of what the formulas call infinite.
+ * g_bias sums dz unrounded.  Outputs that are NULL are left out. */
 typedef struct ssmap_linear_grad_args {
     int32_t dtype;                     /* of x, w, pre and the outputs */
     int32_t grad_dtype;                /* of g: dtype or SSMAP_F32 */

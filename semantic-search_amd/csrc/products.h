@@ -12,7 +12,8 @@ namespace ssmap {
 struct Product {
     int64_t M, N, K;
     int64_t out_batches;                    // out, a, b and the epilogue advance together
-    int64_t sum_batches;                    // the sum runs over this many blocks of K as well (planes: over the envs)
+    int64_t sum_batches;                    // the sum runs over this many blocks of K as well (over the envs, over dz's parts)
+    int64_t b_again;                        // after this many of them b starts over
     const void *a, *b;
     int64_t a_m, a_k, a_out, a_sum;         // strides in elements; of an out batch; of a sum batch
     int64_t b_n, b_k, b_out, b_sum;

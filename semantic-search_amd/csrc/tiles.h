@@ -282,13 +282,15 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
         const char *pa = static_cast<const char *>(p.a) + (e * p.a_out + i0 * p.a_m) * SIZE;
         const char *pb = static_cast<const char *>(p.b) + (e * p.b_out + j0 * p.b_n) * SIZE;
         int64_t at = first % (steps ? steps : 1);      // stage within its sum batch
+        int64_t b_block = first / (steps ? steps : 1) % p.b_again;
         pa += first / (steps ? steps : 1) * p.a_sum * SIZE + at * step_i;
-        pb += first / (steps ? steps : 1) * p.b_sum * SIZE + at * step_j;
+        pb += b_block * p.b_sum * SIZE + at * step_j;
         const auto advance = [&] {
             if (++at == steps) {
                 at = 0;
                 pa += p.a_sum * SIZE - (steps - 1) * step_i;
                 pb += p.b_sum * SIZE - (steps - 1) * step_j;
+                if (++b_block == p.b_again) b_block = 0, pb -= p.b_again * p.b_sum * SIZE;
             } else {
                 pa += step_i;
                 pb += step_j;
@@ -723,13 +725,14 @@ __global__ __launch_bounds__(256) void k_pack(const elem_t<DT> *from, int64_t ba
     }
 }
 
-// Copies one operand (strides: dense across or along the sum) behind p.parts and points at the copy.
+// Copies one operand (strides: dense across or along the sum; `blocks_in_sum` of it) behind p.parts and points at
+// the copy.
 template <int DT>
-void pack_side(const Product &p, int64_t at, bool kc, int64_t rows, const void *&side, int64_t &row, int64_t &k, int64_t &out, int64_t &sum, hipStream_t st) {
+void pack_side(const Product &p, int64_t at, bool kc, int64_t rows, int64_t blocks_in_sum, const void *&side, int64_t &row, int64_t &k, int64_t &out, int64_t &sum, hipStream_t st) {
     if (at < 0) return;
     constexpr int64_t E = 16 / sizeof(elem_t<DT>);
     const int64_t lines = kc ? rows : p.K, dense = kc ? p.K : rows, pitch = (dense + E - 1) / E * E;
-    const int64_t batches = p.sum_batches > 1 ? p.sum_batches : out ? p.out_batches : 1;
+    const int64_t batches = p.sum_batches > 1 ? blocks_in_sum : out ? p.out_batches : 1;
     elem_t<DT> *to = reinterpret_cast<elem_t<DT> *>(reinterpret_cast<char *>(p.parts) + at);
     const int64_t units = batches * lines * (pitch / E);
     k_pack<DT><<<blocks((units + 255) / 256), 256, 0, st>>>(static_cast<const elem_t<DT> *>(side), p.sum_batches > 1 ? sum : out, kc ? row : k, batches, lines, dense,
@@ -744,8 +747,8 @@ template <int DT, int OT>
 void launch_product(Product p, hipStream_t st) {
     if (p.M * p.N * p.out_batches == 0) return;
     const bool ik = p.a_k == 1, jk = p.b_k == 1;
-    pack_side<DT>(p, p.pack_a, ik, p.M, p.a, p.a_m, p.a_k, p.a_out, p.a_sum, st);
-    pack_side<DT>(p, p.pack_b, jk, p.N, p.b, p.b_n, p.b_k, p.b_out, p.b_sum, st);
+    pack_side<DT>(p, p.pack_a, ik, p.M, p.sum_batches, p.a, p.a_m, p.a_k, p.a_out, p.a_sum, st);
+    pack_side<DT>(p, p.pack_b, jk, p.N, p.b_again, p.b, p.b_n, p.b_k, p.b_out, p.b_sum, st);
     if (p.shape == kFewRows) {
         const unsigned n = blocks((p.N + 15) / 16 * p.out_batches);
         if (p.M <= 16) k_few_rows<DT, OT, 1><<<n, kFewWaves * 64, 0, st>>>(p);

@@ -331,8 +331,10 @@ def linear_grad(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, *, ac
                 need_bias: bool = True) -> LinearGrads:
     """Gradients of `linear` with respect to x, weight and bias, all in x's type, from `grad` = dL/dy (x's
     type or float32; it is also the residual's gradient).  With an activation, `pre` is what
-    linear(..., keep_pre=True) returned.  16-bit x: grad act'(pre) is rounded to x's type before the two
-    products, so float16 callers scale their loss as usual."""
+    linear(..., keep_pre=True) returned.  16-bit x: where grad act'(pre) is no value of x's type, the two
+    products sum two parts of it, which hold 16 (bfloat16) or 22 (float16) of its bits and take twice the
+    time; float16 callers scale their loss as usual.  An infinite x or weight can make NaN of what the
+    formula calls infinite."""
     dt, act, dev = _dtype("x", x), _activation(activation), x.device
     outer, inner, w_stride = _weight(x, weight)
     shape = _y_shape(x, outer, planes)

@@ -713,6 +713,47 @@ def test_linear_grad_views_and_parts():
         assert torch.equal(a, c)
 
 
+def check_grad_rounded_once(got, want, size, gsize, n, N, w, x, dtype):
+    """dz counts with 2^-16 (bf16: two roundings of 2^-8) or 2^-22 (fp16: of 2^-11) of its size, after about 16 roundings
+    of values up to |g|; the products sum two parts of it, and the result alone is rounded to 16 bits.  fp16 has steps of
+    2^-24 at the least: what both parts leave of a value of dz is half of one."""
+    keeps = {torch.bfloat16: 2.0 ** -16, torch.float16: 2.0 ** -22, torch.float32: 0.0}[dtype]
+    floor = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    lost = (floor * w.double().abs().sum(0), floor * x.double().abs().reshape(-1, x.shape[-1]).sum(0), 0.0)
+    for i, (k, terms) in enumerate((("x", N), ("weight", n), ("bias", n))):
+        tol = (U * (2 * terms + 8) + keeps) * size[i] * 1.0001 + 24 * U * gsize[i] + lost[i] + HALF[dtype] * want[i].abs() * 1.0001 + SMALLEST[dtype]
+        close("gradient of " + k, getattr(got, k), want[i].cpu(), tol.cpu())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("lead,K,N,planes", [((1,), 1, 1, False), ((70,), 72, 130, False), ((300,), 96, 65, False), ((515,), 264, 136, False),
+                                             ((1,), 515, 400, False), ((2, 16, 20), 256, 40, True), ((2, 513), 130, 21, True), ((3, 1), 8, 1, True)])
+def test_linear_grad_is_rounded_once(lead, K, N, planes, dtype):
+    """A gradient in float32, and one that an activation's slope multiplies, reach the products unrounded."""
+    for act, out in ((None, torch.float32), ("gelu", dtype), ("relu", dtype), ("silu", torch.float32)):
+        x, w, _, g = make_linear(lead, K, N, dtype, out, K + N, planes=planes)
+        pre = (torch.randn(g.shape, generator=gen(K)) * 1.5).to(dtype) if act else None
+        got = ssa.linear_grad(g.cuda(), x.cuda(), w.cuda(), activation=act, pre=None if pre is None else pre.cuda(), planes=planes)
+        want, size, gsize = plain_linear_grad(g, x, w, act, pre, planes)
+        check_grad_rounded_once(got, want, size, gsize, x[..., 0].numel(), N, w, x, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("B,n,K,N,planes", [(1, 8190, 1000, 4088, False), (2, 701, 1001, 603, False), (3, 701, 1001, 603, True),
+                                            (2, 3000, 512, 520, False), (2, 20000, 64, 40, True)])
+def test_large_linear_grad_is_rounded_once(B, n, K, N, planes, dtype):
+    """The largest tiles, split sums, copied operands and batches that do not merge, against 64-bit products."""
+    g = torch.Generator(device="cuda").manual_seed(K)
+    x = torch.full((B, n + 1, K), math.nan, device="cuda", dtype=dtype)[:, :n]
+    x.copy_(torch.randn((B, n, K), device="cuda", generator=g))
+    w = (torch.randn((N, K), device="cuda", generator=g) / math.sqrt(K)).to(dtype)
+    dy = torch.randn((B, N, n) if planes else (B, n, N), device="cuda", generator=g).to(dtype)
+    pre = (torch.randn(dy.shape, device="cuda", generator=g) * 1.5).to(dtype)
+    got = ssa.linear_grad(dy, x, w, activation="silu", pre=pre, planes=planes)
+    want, size, gsize = plain_linear_grad(dy, x, w, "silu", pre, planes)
+    check_grad_rounded_once(got, want, size, gsize, B * n, N, w, x, dtype)
+
+
 # ------------------------------------------------------------------ together, streams, graphs, the engine
 
 def test_a_training_step_of_a_head():
