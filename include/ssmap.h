@@ -384,7 +384,8 @@ int ssmap_linear(const ssmap_linear_args *args, void *stream);
  *   g_x = dz w,   g_w = dz^T x,   g_bias = sum of dz over the positions   (g itself is the residual's).
  * Where dtype has 16 bits and g is float32 or an activation is given, dz goes into the two products as two values of
  * dtype, the rounded one and what the rounding left (the matrix instructions' operands have no more bits): 16 bits of
- * it for SSMAP_BF16, 22 for SSMAP_F16.  An infinite x or w then can make NaN of what the formulas call infinite.
+ * it for SSMAP_BF16, 22 for SSMAP_F16, there scaled by the power of two that the largest finite |g| asks for (what lies
+ * below 2^-38 of that is lost).  An infinite x or w then can make NaN of what the formulas call infinite.
  * g_bias sums dz unrounded.  Outputs that are NULL are left out. */
 typedef struct ssmap_linear_grad_args {
     int32_t dtype;                     /* of x, w, pre and the outputs */

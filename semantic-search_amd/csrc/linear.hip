@@ -29,6 +29,10 @@ inline bool direct_side(const void *p, int64_t line, int64_t out, int64_t sum, i
 // forward product's is.  With the rounded value alone the gradients' distance to the definition grows by 1.4 (8192 x
 // 4096 x 4096 bf16 with gelu: 2.35e-3 against 1.66e-3 of the results' size) and the products take half the time (the
 // whole call 494 against 930 us).
+//
+// fp16 holds nothing above 65504 and little below 2^-14, where a float32 gradient averaged over a frame's positions
+// lies.  There dz is multiplied by the power of two that brings the largest finite |g| to 2^13 ... 2^14 (no slope exceeds
+// 1.13), and the products' sums by its inverse: what is lost of a value is at most 2^-38 of that largest one.
 constexpr int kDzRows = 128;       // rows: positions a block sums; 8 threads down, 32 packs of 8 outputs across
 constexpr int kDzPlane = 16384;    // planes: positions a block sums
 
@@ -46,7 +50,7 @@ __device__ __forceinline__ void load8(const elem_t<T> *p, int left, float (&v)[8
     }
 }
 template <bool WHOLE, int DT, int OT>
-__device__ __forceinline__ void dz_pack(const elem_t<OT> *g, const elem_t<DT> *pre, elem_t<DT> *dz, int64_t rest, int left, int room, int act, float (&sum)[8]) {   // room: of dz's line, zeros included
+__device__ __forceinline__ void dz_pack(const elem_t<OT> *g, const elem_t<DT> *pre, elem_t<DT> *dz, int64_t rest, float by, int left, int room, int act, float (&sum)[8]) {   // room: of dz's line, zeros included
     float v[8];
     load8<WHOLE, OT>(g, left, v);
     if (pre) {
@@ -79,6 +83,7 @@ __device__ __forceinline__ void dz_pack(const elem_t<OT> *g, const elem_t<DT> *p
     constexpr float most = DT == SSMAP_BF16 ? 0x1.fep127f : 65504.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
+        if constexpr (DT == SSMAP_F16) v[e] *= by;
         w[e] = Elem<DT>::put(fminf(fmaxf(v[e], -most), most));
         v[e] -= Elem<DT>::get(w[e]);
     }
@@ -88,10 +93,49 @@ __device__ __forceinline__ void dz_pack(const elem_t<OT> *g, const elem_t<DT> *p
     keep(dz + rest);
 }
 
+// The largest finite |g| of each block's share: lines of `dense` values, `lines` a batch.
+constexpr int kPeaks = 1024;   // blocks at most
+template <int OT>
+__global__ __launch_bounds__(256) void k_peak(int64_t batch, int64_t lines, int64_t dense, const elem_t<OT> *g, int64_t g_batch, int64_t g_line, float *peaks) {
+    __shared__ float part[4];
+    const int64_t per = (dense + 7) / 8, units = batch * lines * per;
+    float peak = 0.0f;
+    for (int64_t u = blockIdx.x * 256ll + threadIdx.x; u < units; u += gridDim.x * 256ll) {
+        const int64_t l = u / per, c = u % per * 8;
+        const elem_t<OT> *p = g + l / lines * g_batch + l % lines * g_line + c;
+        float v[8];
+        if (c + 8 <= dense) load8<true, OT>(p, 8, v);
+        else load8<false, OT>(p, (int)(dense - c), v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) peak = fabsf(v[e]) < INFINITY ? fmaxf(peak, fabsf(v[e])) : peak;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) peak = fmaxf(peak, __shfl_xor(peak, d));
+    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = peak;
+    __syncthreads();
+    if (!threadIdx.x) peaks[blockIdx.x] = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+}
+// scale[0]: what dz is multiplied by, scale[1]: its inverse.  One block.
+__global__ __launch_bounds__(kPeaks) void k_scale(const float *peaks, int n, float *scale) {
+    __shared__ float part[kPeaks / 64];
+    float peak = threadIdx.x < n ? peaks[threadIdx.x] : 0.0f;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) peak = fmaxf(peak, __shfl_xor(peak, d));
+    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = peak;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int k = 1; k < kPeaks / 64; ++k) peak = fmaxf(peak, part[k]);
+    const int e = (int)(__builtin_bit_cast(uint32_t, peak) >> 23) - 127;   // floor(log2 peak), -127 below the normal ones
+    const int by = 13 - e < 126 ? 13 - e : 126;                            // -114 ... 126: both powers are normal
+    scale[0] = __builtin_bit_cast(float, (uint32_t)(127 + by) << 23);
+    scale[1] = __builtin_bit_cast(float, (uint32_t)(127 - by) << 23);
+}
+
 // sums[batch * row chunks][outer]; `rest`: what the roundings left lies that many values behind, or 0
 template <int DT, int OT>
 __global__ __launch_bounds__(256) void k_dz_rows(int64_t batch, int64_t rows, int64_t outer, const elem_t<OT> *g, int64_t g_batch, int64_t g_row,
-                                                 const elem_t<DT> *pre, int act, elem_t<DT> *dz, int64_t dz_line, int64_t rest, float *sums) {
+                                                 const elem_t<DT> *pre, int act, elem_t<DT> *dz, int64_t dz_line, int64_t rest, const float *scale, float *sums) {
+    const float by = scale ? *scale : 1.0f;
     __shared__ float part[8][256];
     const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
     const int64_t strips = (outer + 255) / 256, chunks = (rows + kDzRows - 1) / kDzRows;
@@ -104,7 +148,7 @@ __global__ __launch_bounds__(256) void k_dz_rows(int64_t batch, int64_t rows, in
 #pragma unroll 2
             for (int64_t r = r0 + ty; r < end; r += 8) {
                 const int64_t o = (b * rows + r) * outer + n;
-                dz_pack<whole.value, DT, OT>(g + b * g_batch + r * g_row + n, pre ? pre + o : nullptr, dz ? dz + (b * rows + r) * dz_line + n : nullptr, rest, left, (int)(dz_line - n < 8 ? dz_line - n : 8), act, sum);
+                dz_pack<whole.value, DT, OT>(g + b * g_batch + r * g_row + n, pre ? pre + o : nullptr, dz ? dz + (b * rows + r) * dz_line + n : nullptr, rest, by, left, (int)(dz_line - n < 8 ? dz_line - n : 8), act, sum);
             }
         };
         if (unit % strips * 256 + 256 <= outer) walk(std::true_type{});
@@ -125,7 +169,8 @@ __global__ __launch_bounds__(256) void k_dz_rows(int64_t batch, int64_t rows, in
 // sums[batch * chunks][outer]
 template <int DT, int OT>
 __global__ __launch_bounds__(256) void k_dz_planes(int64_t batch, int64_t rows, int64_t outer, const elem_t<OT> *g, int64_t g_batch, int64_t g_plane,
-                                                   const elem_t<DT> *pre, int act, elem_t<DT> *dz, int64_t dz_line, int64_t rest, float *sums) {
+                                                   const elem_t<DT> *pre, int act, elem_t<DT> *dz, int64_t dz_line, int64_t rest, const float *scale, float *sums) {
+    const float by = scale ? *scale : 1.0f;
     __shared__ float part[256];
     const int64_t chunks = (rows + kDzPlane - 1) / kDzPlane;
     for (int64_t unit = blockIdx.x; unit < chunks * outer * batch; unit += gridDim.x) {
@@ -139,10 +184,10 @@ __global__ __launch_bounds__(256) void k_dz_planes(int64_t batch, int64_t rows, 
 #pragma unroll 2
         for (; r + 2048 <= end; r += 2048) {
             const int64_t at = r + threadIdx.x * 8;
-            dz_pack<true, DT, OT>(gp + at, zp ? zp + at : nullptr, dp ? dp + at : nullptr, rest, 8, 8, act, sum);
+            dz_pack<true, DT, OT>(gp + at, zp ? zp + at : nullptr, dp ? dp + at : nullptr, rest, by, 8, 8, act, sum);
         }
         const int64_t at = r + threadIdx.x * 8;
-        if (at < end) dz_pack<false, DT, OT>(gp + at, zp ? zp + at : nullptr, dp ? dp + at : nullptr, rest, (int)(end - at < 8 ? end - at : 8),
+        if (at < end) dz_pack<false, DT, OT>(gp + at, zp ? zp + at : nullptr, dp ? dp + at : nullptr, rest, by, (int)(end - at < 8 ? end - at : 8),
                                            (int)(end < rows ? 8 : dz_line - at < 8 ? dz_line - at : 8), act, sum);
         if (!sums) continue;
         part[threadIdx.x] = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
@@ -206,15 +251,16 @@ int check_grad(const ssmap_linear_grad_args *a) {
     return check(a, a->grad_dtype);
 }
 
-// The workspace of ssmap_linear_grad: dz, the bias's sums, the partial results of the products (one after
-// the other, so they share a place).
+// The workspace of ssmap_linear_grad: dz, its scale and the blocks' peaks, the bias's sums, the partial results of the
+// products (one after the other, so they share a place).
 struct GradPlan {
     bool planes, copies;               // copies: dz is not g itself
     int64_t dz_line;                   // values a line of dz takes: a multiple of 16 bytes, zeros behind the dense ones
     int64_t dz_rest;                   // values from dz to what its roundings left; 0: dz is exact
     int64_t chunks;                    // sums a block leaves for each output
     Product x, w;
-    int64_t dz_bytes, sum_bytes, part_bytes;
+    int64_t dz_bytes, scale_bytes, sum_bytes, part_bytes;
+    int64_t bytes() const { return dz_bytes + scale_bytes + sum_bytes + part_bytes; }
 };
 
 inline int64_t aligned(int64_t bytes) { return (bytes + 255) & ~(int64_t)255; }
@@ -253,6 +299,7 @@ GradPlan plan_grad(const ssmap_linear_grad_args *a) {
     q.dz_rest = a->dtype != SSMAP_F32 && (a->activation != SSMAP_ACT_NONE || a->grad_dtype != a->dtype) ? values : 0;
     const int64_t parts = q.dz_rest ? 2 : 1;
     q.dz_bytes = q.copies && (a->g_x || a->g_w) ? aligned(parts * values * size) : 0;
+    q.scale_bytes = q.dz_bytes && q.dz_rest && a->dtype == SSMAP_F16 ? aligned((2 + kPeaks) * 4) : 0;
     q.sum_bytes = a->g_bias ? aligned(q.chunks * a->outer * 4) : 0;
     // dz: [part][batch][position][output] or [part][batch][output][position]
     const void *dz = q.copies ? a->workspace : a->g;
@@ -300,7 +347,7 @@ int ssmap_linear(const ssmap_linear_args *a, void *stream) {
 int64_t ssmap_linear_grad_workspace(const ssmap_linear_grad_args *a) {
     if (check_grad(a) != SSMAP_OK) return -1;
     const GradPlan q = plan_grad(a);
-    return q.dz_bytes + q.sum_bytes + q.part_bytes;
+    return q.bytes();
 }
 
 int ssmap_linear_grad(const ssmap_linear_grad_args *a, void *stream) {
@@ -311,23 +358,32 @@ int ssmap_linear_grad(const ssmap_linear_grad_args *a, void *stream) {
     if ((a->g_x && positions && a->inner && a->outer && !a->w) || (a->g_w && a->outer && a->inner && positions && !a->x))
         return head_error(SSMAP_ERR_INVALID_ARG, "null argument");
     GradPlan q = plan_grad(a);
-    const int64_t need = q.dz_bytes + q.sum_bytes + q.part_bytes;
+    const int64_t need = q.bytes();
     if (a->workspace_bytes < need || (need && (!a->workspace || reinterpret_cast<uintptr_t>(a->workspace) % 16)))
         return head_error(SSMAP_ERR_INVALID_ARG, "the workspace is not at a multiple of 16 or smaller than ssmap_linear_grad_workspace says");
     const hipStream_t st = static_cast<hipStream_t>(stream);
     char *ws = static_cast<char *>(a->workspace);
-    float *sums = q.sum_bytes ? reinterpret_cast<float *>(ws + q.dz_bytes) : nullptr;
-    q.x.parts = q.w.parts = reinterpret_cast<float *>(ws + q.dz_bytes + q.sum_bytes);
+    float *scale = q.scale_bytes ? reinterpret_cast<float *>(ws + q.dz_bytes) : nullptr;
+    float *sums = q.sum_bytes ? reinterpret_cast<float *>(ws + q.dz_bytes + q.scale_bytes) : nullptr;
+    q.x.parts = q.w.parts = reinterpret_cast<float *>(ws + q.bytes() - q.part_bytes);
+    q.x.unscale = q.w.unscale = scale && positions && a->outer ? scale + 1 : nullptr;   // without a dz nobody writes it
     with_types(a->dtype, a->grad_dtype, [&](auto dt, auto ot) {
         constexpr int DT = dt.value, OT = ot.value;
         const auto *g = static_cast<const elem_t<OT> *>(a->g);
         const auto *pre = a->activation == SSMAP_ACT_NONE ? nullptr : static_cast<const elem_t<DT> *>(a->pre);
         auto *dz = q.dz_bytes ? reinterpret_cast<elem_t<DT> *>(ws) : nullptr;
+        if (q.x.unscale) {
+            const int64_t lines = q.planes ? a->outer : a->rows, dense = q.planes ? a->rows : a->outer;
+            const int64_t want = (a->batch * lines * ((dense + 7) / 8) + 255) / 256;
+            const unsigned n = (unsigned)(want < kPeaks ? want : kPeaks);
+            k_peak<OT><<<n, 256, 0, st>>>(a->batch, lines, dense, g, a->g_batch_stride, a->g_inner_stride, scale + 2);
+            k_scale<<<1, kPeaks, 0, st>>>(scale + 2, (int)n, scale);
+        }
         if (positions * a->outer && (dz || sums)) {
             if (q.planes)
-                k_dz_planes<DT, OT><<<blocks(q.chunks * a->outer), 256, 0, st>>>(a->batch, a->rows, a->outer, g, a->g_batch_stride, a->g_inner_stride, pre, a->activation, dz, q.dz_line, q.dz_rest, sums);
+                k_dz_planes<DT, OT><<<blocks(q.chunks * a->outer), 256, 0, st>>>(a->batch, a->rows, a->outer, g, a->g_batch_stride, a->g_inner_stride, pre, a->activation, dz, q.dz_line, q.dz_rest, scale, sums);
             else
-                k_dz_rows<DT, OT><<<blocks(q.chunks * ((a->outer + 255) / 256)), 256, 0, st>>>(a->batch, a->rows, a->outer, g, a->g_batch_stride, a->g_inner_stride, pre, a->activation, dz, q.dz_line, q.dz_rest, sums);
+                k_dz_rows<DT, OT><<<blocks(q.chunks * ((a->outer + 255) / 256)), 256, 0, st>>>(a->batch, a->rows, a->outer, g, a->g_batch_stride, a->g_inner_stride, pre, a->activation, dz, q.dz_line, q.dz_rest, scale, sums);
         }
         if (a->g_bias && a->outer) k_bias_grad<DT><<<blocks((a->outer + 3) / 4), 256, 0, st>>>(q.chunks, a->outer, sums, static_cast<elem_t<DT> *>(a->g_bias));
         if (a->g_x) launch_product<DT, DT>(q.x, st);

@@ -19,6 +19,7 @@ struct Product {
     int64_t b_n, b_k, b_out, b_sum;
     void *out;                              // dense [out_batches][M][N]
     void *pre;                              // the same in the operands' type, or NULL
+    const float *unscale;                   // fp16: the products' sums are multiplied by this, on the device; or NULL
     const void *bias, *res;
     int32_t bias_f32, bias_along_m, act, pad;
     int64_t res_out, res_m;

@@ -223,6 +223,11 @@ __device__ __forceinline__ void load_bias(const Product &p, int64_t m, int64_t n
 // `o` is the first result's place in the dense output.
 template <bool WHOLE, int DT, int OT, int N, bool PAST = false>
 __device__ __forceinline__ void finish(const Product &p, int64_t o, int left, float (&z)[N], const float (&bias)[N], const Run<OT, N> &res) {
+    if constexpr (DT == SSMAP_F16 && OT == SSMAP_F16)
+        if (p.unscale) {
+#pragma unroll
+            for (int q = 0; q < N; ++q) z[q] *= *p.unscale;
+        }
     if (p.bias) {
 #pragma unroll
         for (int q = 0; q < N; ++q) z[q] += bias[q];

@@ -333,7 +333,8 @@ def linear_grad(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, *, ac
     type or float32; it is also the residual's gradient).  With an activation, `pre` is what
     linear(..., keep_pre=True) returned.  16-bit x: where grad act'(pre) is no value of x's type, the two
     products sum two parts of it, which hold 16 (bfloat16) or 22 (float16) of its bits and take twice the
-    time; float16 callers scale their loss as usual.  An infinite x or weight can make NaN of what the
+    time; float16 values are scaled for it by the power of two that the largest finite |grad| asks for, so
+    that only what lies below 2^-38 of that is lost.  An infinite x or weight can make NaN of what the
     formula calls infinite."""
     dt, act, dev = _dtype("x", x), _activation(activation), x.device
     outer, inner, w_stride = _weight(x, weight)

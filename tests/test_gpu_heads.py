@@ -754,6 +754,48 @@ def test_large_linear_grad_is_rounded_once(B, n, K, N, planes, dtype):
     check_grad_rounded_once(got, want, size, gsize, B * n, N, w, x, dtype)
 
 
+@pytest.mark.parametrize("planes", [False, True])
+@pytest.mark.parametrize("size,scale", [(1e-12, 6e4), (1e-9, 3e4), (3e-7, 500.0), (1e-3, 1.0), (3e4, 1e-3), (1e7, 1e-4), (1e8, 1e-5)])
+def test_linear_grad_of_float16_holds_any_float32_gradient(size, scale, planes):
+    """Gradients far below and above what fp16 holds, into results that it does hold; an activation's slope on top."""
+    B, n, K, N = 2, 150, 72, 64
+    for act in (None, "gelu"):
+        x, w, _, g = make_linear((B, n), K, N, torch.float16, torch.float32, 3, planes=planes)
+        x, w, g = (x.float() * scale / 8).half(), (w.float() * scale).half(), g * size
+        pre = (torch.randn(g.shape, generator=gen(K)) * 1.5).half() if act else None
+        got = ssa.linear_grad(g.cuda(), x.cuda(), w.cuda(), activation=act, pre=None if pre is None else pre.cuda(), planes=planes)
+        want, mag, gsize = plain_linear_grad(g, x, w, act, pre, planes)
+        peak = float(g.abs().max())
+        lost = (w.double().abs().sum(0), x.double().abs().reshape(-1, K).sum(0))
+        for i, (k, terms) in enumerate((("x", N), ("weight", B * n))):
+            # two roundings of 2^-11, sums of two parts, the slope's 16 roundings, 2^-38 of the peak a value, the result
+            tol = (U * (2 * terms + 8) + 2.0 ** -22) * mag[i] * 1.0001 + 24 * U * gsize[i] + 2.0 ** -38 * peak * lost[i] + HALF[torch.float16] * want[i].abs() * 1.0001 + 2.0 ** -25
+            close("gradient of " + k, getattr(got, k), want[i], tol)
+            assert float(getattr(got, k).abs().max()) > 0
+
+
+@pytest.mark.parametrize("planes", [False, True])
+def test_linear_grad_of_float16_scales_by_finite_values(planes):
+    """Infinities and NaN of a gradient stay in their positions and leave the scale alone; zeros stay zeros."""
+    B, n, K, N = 2, 40, 24, 16
+    x, w, _, g = make_linear((B, n), K, N, torch.float16, torch.float32, 4, planes=planes)
+    w = w.abs() + 0.01
+    g = g * 1e-6
+    clean = ssa.linear_grad(g.cuda(), x.cuda(), w.cuda(), planes=planes, need_weight=False)
+    bad = g.clone()
+    at = (lambda e, r, o: (e, o, r)) if planes else (lambda e, r, o: (e, r, o))
+    bad[at(0, 3, 5)], bad[at(1, 7, 2)] = math.inf, math.nan
+    got = ssa.linear_grad(bad.cuda(), x.cuda(), w.cuda(), planes=planes)
+    assert (got.x[0, 3] == math.inf).all() and torch.isnan(got.x[1, 7]).all()
+    keep = torch.ones((B, n), dtype=torch.bool)
+    keep[0, 3] = keep[1, 7] = False
+    assert float(clean.x.abs().max()) > 0 and torch.equal(got.x.cpu()[keep], clean.x.cpu()[keep])
+    others = [o for o in range(N) if o not in (2, 5)]
+    assert torch.isfinite(got.weight[others]).all() and torch.isfinite(got.bias[others]).all()
+    for t in ssa.linear_grad(torch.zeros_like(g).cuda(), x.cuda(), w.cuda(), planes=planes):
+        assert not t.any()
+
+
 # ------------------------------------------------------------------ together, streams, graphs, the engine
 
 def test_a_training_step_of_a_head():
