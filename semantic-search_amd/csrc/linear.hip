@@ -269,6 +269,7 @@ Product forward_product(const ssmap_linear_args *a) {
     const bool planes = a->layout == SSMAP_PLANES;
     Product p{};
     p.K = a->inner; p.out_batches = a->batch; p.sum_batches = p.b_again = 1;
+    p.a_sums = p.b_sums = true;
     p.out = a->y; p.pre = a->pre; p.bias = a->bias; p.res = a->residual;
     p.bias_f32 = a->bias_dtype == SSMAP_F32; p.bias_along_m = planes; p.act = a->activation;
     p.res_out = a->res_batch_stride; p.res_m = a->res_inner_stride;
@@ -308,6 +309,7 @@ GradPlan plan_grad(const ssmap_linear_grad_args *a) {
     Product &x = q.x, &w = q.w;
     x.M = a->rows; x.N = a->inner; x.K = a->outer; x.out_batches = a->batch; x.sum_batches = parts; x.b_again = 1;
     x.a_pads = w.a_pads = q.copies;
+    x.a_sums = !q.planes; w.a_sums = q.planes;   // b's dense axis is x's features: the result's
     x.a = dz; x.a_out = batch; x.a_sum = q.dz_rest; x.a_m = to_row; x.a_k = to_out;
     x.b = a->w; x.b_n = 1; x.b_k = a->w_row_stride;
     x.out = a->g_x;
@@ -396,7 +398,13 @@ int ssmap_linear_grad(const ssmap_linear_grad_args *a, void *stream) {
 
 int64_t ssmap::plan_product(Product &p, int dtype) {
     const int size = head_dtype_size(dtype);
-    const bool ik = p.a_k == 1, jk = p.b_k == 1;
+    const bool ik = p.a_sums, jk = p.b_sums;
+    // a line that stands alone has no stride
+    if ((ik ? p.M : p.K) == 1) (ik ? p.a_m : p.a_k) = 0;
+    if ((jk ? p.N : p.K) == 1) (jk ? p.b_n : p.b_k) = 0;
+    if (p.out_batches == 1) p.a_out = p.b_out = 0;
+    if (p.sum_batches == 1) p.a_sum = 0;
+    if (p.b_again == 1) p.b_sum = 0;
     p.splits = 1;
     p.pack_a = p.pack_b = -1;
     const int64_t steps = (p.K * size + 127) / 128 * p.sum_batches;

@@ -17,6 +17,10 @@ struct Product {
     const void *a, *b;
     int64_t a_m, a_k, a_out, a_sum;         // strides in elements; of an out batch; of a sum batch
     int64_t b_n, b_k, b_out, b_sum;
+    // Which axis of an operand is dense in memory (its stride is 1): the sum's, or the result's.  The builder says so;
+    // strides cannot, as overlapping or single lines may have a stride of 1 along both.  b is dense along the sum only
+    // where a is: those three forms have kernels.
+    bool a_sums, b_sums;
     void *out;                              // dense [out_batches][M][N]
     void *pre;                              // the same in the operands' type, or NULL
     const float *unscale;                   // fp16: the products' sums are multiplied by this, on the device; or NULL

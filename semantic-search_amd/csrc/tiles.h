@@ -751,7 +751,7 @@ void pack_side(const Product &p, int64_t at, bool kc, int64_t rows, int64_t bloc
 template <int DT, int OT>
 void launch_product(Product p, hipStream_t st) {
     if (p.M * p.N * p.out_batches == 0) return;
-    const bool ik = p.a_k == 1, jk = p.b_k == 1;
+    const bool ik = p.a_sums, jk = p.b_sums;
     pack_side<DT>(p, p.pack_a, ik, p.M, p.sum_batches, p.a, p.a_m, p.a_k, p.a_out, p.a_sum, st);
     pack_side<DT>(p, p.pack_b, jk, p.N, p.b_again, p.b, p.b_n, p.b_k, p.b_out, p.b_sum, st);
     if (p.shape == kFewRows) {

@@ -796,6 +796,49 @@ def test_linear_grad_of_float16_scales_by_finite_values(planes):
         assert not t.any()
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("K,N,n", [(65, 3, 40), (512, 512, 8191), (513, 70, 33000)])
+def test_linear_of_sliding_windows(K, N, n, dtype):
+    """Rows that overlap, one element on from each other, have a stride of 1 along both axes: features x and
+    weights, forward and backward, below and above the size from which operands are copied."""
+    g = torch.Generator(device="cuda").manual_seed(K)
+    x = torch.randn(n + K - 1, device="cuda", generator=g).to(dtype).unfold(0, K, 1)
+    dense = (torch.randn((N, K), device="cuda", generator=g) / math.sqrt(K)).to(dtype)
+    slid = (torch.randn(N + K - 1, device="cuda", generator=g) / math.sqrt(K)).to(dtype).unfold(0, K, 1)
+    assert x.stride() == (1, 1) and slid.stride() == (1, 1)
+    dy = torch.randn((n, N), device="cuda", generator=g).to(dtype)
+    d, xd = dy.double(), x.double()
+    for w in (dense, slid):
+        wd = w.double()
+        tol = lambda want, size, terms: (U * (terms + 8) * size * 1.0001 + HALF[dtype] * want.abs() * 1.0001 + SMALLEST[dtype]).cpu()  # noqa: E731
+        for planes in (False, True):
+            move = (lambda t: t.t()[None].contiguous()) if planes else (lambda t: t)
+            feat = x[None] if planes else x
+            want, size = move(xd @ wd.t()), move(xd.abs() @ wd.abs().t())
+            close("y", ssa.linear(feat, w, planes=planes), want.cpu(), tol(want, size, K))
+            got = ssa.linear_grad(move(dy), feat, w, planes=planes)
+            want, size = d @ wd, d.abs() @ wd.abs()
+            close("gradient of x", got.x.view(n, K), want.cpu(), tol(want, size, N))
+            want, size = d.t() @ xd, d.abs().t() @ xd.abs()
+            close("gradient of weight", got.weight, want.cpu(), tol(want, size, n))
+
+
+def test_linear_grad_of_a_single_class_whose_weight_is_a_turned_column():
+    """[1, D] made by .t() is contiguous and has strides (1, 1).  One product a result: one rounding of it, in a
+    product large enough that out of line operands are copied."""
+    E, n, D = 4, 1 << 20, 256
+    w = torch.randn((D, 1), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).bfloat16().t()
+    assert w.is_contiguous() and w.stride() == (1, 1)
+    x = torch.zeros((E, n, D), dtype=torch.bfloat16, device="cuda")
+    dy = torch.randn((E, 1, n), device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).bfloat16()
+    got = ssa.linear_grad(dy, x, w, planes=True, need_weight=False, need_bias=False)
+    assert torch.equal(got.x, dy.transpose(1, 2) * w)
+    x = x[:1].float()
+    dy = dy[:1].float()
+    got = ssa.linear_grad(dy, x, w.float(), planes=True, need_weight=False, need_bias=False)
+    assert torch.equal(got.x, dy.transpose(1, 2) * w.float())
+
+
 # ------------------------------------------------------------------ together, streams, graphs, the engine
 
 def test_a_training_step_of_a_head():

@@ -154,3 +154,23 @@ def test_empty_calls_do_nothing():
 def test_struct_sizes():
     c = ssa._capi
     assert [ctypes.sizeof(t) for t in (c.LogProbsArgs, c.LogProbsGradArgs, c.LinearArgs, c.LinearGradArgs)] == [168, 168, 160, 160]
+
+
+def _grad_workspace(**over):
+    p = ctypes.cast(ctypes.create_string_buffer(64), ctypes.c_void_p).value // 16 * 16
+    kw = dict(dtype=1, grad_dtype=1, batch=1, x=p, w=p, g=p)
+    kw.update(over)
+    return ssa._capi.load().ssmap_linear_grad_workspace(ctypes.byref(ssa._capi.LinearGradArgs(**kw)))
+
+
+def test_the_dense_axis_of_an_operand_is_not_read_from_its_strides():
+    """Rows one element apart are dense along both axes; the gradients' products read them along the features, and
+    that is what a copy of them lays out: 8191 lines of 512 values, and not 512 of 8191 (filled up to 8192)."""
+    rows = dict(layout=0, rows=8191, inner=512, outer=512, g_inner_stride=512, w_row_stride=512, g_w=16)
+    assert _grad_workspace(**rows, x_row_stride=1) - _grad_workspace(**rows, x_row_stride=512) == 8191 * 512 * 2
+    planes = dict(layout=1, rows=80000, inner=512, outer=41, g_inner_stride=80000, x_row_stride=512, g_x=16)
+    assert _grad_workspace(**planes, w_row_stride=1) - _grad_workspace(**planes, w_row_stride=512) == 41 * 512 * 2
+    # a line that stands alone has no stride
+    one = dict(layout=1, batch=16, rows=307200, inner=256, outer=1, g_batch_stride=307200, g_inner_stride=307200,
+               x_batch_stride=307200 * 256, x_row_stride=256, g_x=16)
+    assert _grad_workspace(**one, w_row_stride=1) == _grad_workspace(**one, w_row_stride=256) == 0
