@@ -52,14 +52,18 @@ inline unsigned blocks(int64_t n) { return (unsigned)(n < 1 ? 1 : n < (1 << 20) 
 // Chooses p.shape, p.splits, p.part_steps and the copies by sizes, strides and alignment; returns the bytes that
 // p.parts needs.
 int64_t plan_product(Product &p, int dtype);
-// FINE: for results in float32.  Results of 16 bits take erfc from Abramowitz and Stegun's formula 7.1.26,
-// whose error of 1.5e-7 is far below their rounding.
+// FINE: for results in float32.  Results of 16 bits take erfc(x) exp(x^2) / 2 = t P(t) with t = 1 / (1 + 0.5125 x), a
+// least-maximum fit relative to the value over 0 <= x <= 10: it is off by at most 7.7e-7 of it, and by 1.7e-5 with the
+// rounding of x^2 at z = -13, which is far below the rounding of the results (2^-11, 2^-8) out to the smallest of them.
+constexpr float kErfcAt = 0.5125f;
+__device__ __forceinline__ float erfc_ratio(float t) {
+    return t * (0.14465798f + t * (0.142883733f + t * (0.13929078f + t * (0.029507799f + t * (0.17541796f + t * (-0.179791331f + t * 0.0480334461f))))));
+}
 template <bool FINE>
 __device__ __forceinline__ float half_erfc(float x) {   // erfc(x) / 2
     if constexpr (FINE) return 0.5f * erfcf(x);
-    const float a = fabsf(x), t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * a);
-    const float y = t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f))));
-    const float v = y * __builtin_amdgcn_exp2f(-1.44269504088896341f * a * a);
+    const float a = fabsf(x), t = __builtin_amdgcn_rcpf(1.0f + kErfcAt * a);
+    const float v = erfc_ratio(t) * __builtin_amdgcn_exp2f(-1.44269504088896341f * a * a);
     return x < 0.0f ? 1.0f - v : v;
 }
 template <bool FINE>
@@ -82,9 +86,9 @@ __device__ __forceinline__ float slope(float z) {
     if constexpr (ACT == SSMAP_ACT_GELU) {
         if constexpr (FINE) return half_erfc<true>(-0.70710678118654752f * z) + z * 0.39894228040143268f * expf(-0.5f * z * z);
         // the formula of half_erfc at z / sqrt 2: its exponential is the bell
-        const float a = fabsf(z), t = __builtin_amdgcn_rcpf(1.0f + 0.23164188826636f * a);
+        const float a = fabsf(z), t = __builtin_amdgcn_rcpf(1.0f + kErfcAt * 0.70710678118654752f * a);
         const float bell = __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
-        const float tail = bell * t * (0.127414796f + t * (-0.142248368f + t * (0.7107068705f + t * (-0.7265760135f + t * 0.5307027145f))));
+        const float tail = bell * erfc_ratio(t);
         return (z < 0.0f ? tail : 1.0f - tail) + z * 0.39894228040143268f * bell;
     }
     if constexpr (ACT == SSMAP_ACT_GELU_TANH) {

@@ -632,6 +632,24 @@ def test_linear_lets_infinities_and_nan_through():
         assert torch.isfinite(got[keep]).all()
 
 
+@pytest.mark.parametrize("dtype,far", [(torch.bfloat16, 12.5), (torch.float16, 5.25)], ids=ids_of)
+def test_gelu_tail_of_16_bit_results(dtype, far):
+    """gelu and its slope relative to their own size, every value of the type between -far and far.  The formula is off
+    by 7.7e-7 (13 U), the exponential by three roundings of z^2 / 2, sixteen operations around them; the slope's dz holds
+    2^-16 of it.  The slope is a sum of two terms of opposite sign: its errors go by their sizes."""
+    bits = torch.arange(-32768, 32768, dtype=torch.int32).to(torch.int16).view(dtype)
+    z = bits[(bits.float().abs() <= far) & (bits.float().abs() >= 2.0 ** -10)].reshape(-1, 1)
+    one = torch.ones((1, 1), dtype=dtype, device="cuda")
+    zd = z.double()
+    phi, bell = torch.special.erfc(-zd / math.sqrt(2)) / 2, zd * torch.exp(-zd * zd / 2) / math.sqrt(2 * math.pi)
+    rel = U * (32 + 2 * zd * zd)
+    want = zd * phi
+    close("gelu", ssa.linear(z.cuda(), one, activation="gelu"), want, (rel + HALF[dtype] * 1.0001) * want.abs() + SMALLEST[dtype])
+    got = ssa.linear_grad(torch.ones_like(z).cuda(), z.cuda(), one, activation="gelu", pre=z.cuda(), need_weight=False, need_bias=False)
+    want = phi + bell
+    close("slope", got.x, want, (rel + 2.0 ** -16) * (phi + bell.abs()) + HALF[dtype] * want.abs() * 1.0001 + SMALLEST[dtype])
+
+
 def plain_linear_grad(g, x, w, act, pre, planes):
     dz = g.double()
     slope = torch.ones_like(dz)
