@@ -84,12 +84,16 @@ template <int ACT, bool FINE>
 __device__ __forceinline__ float slope(float z) {
     if constexpr (ACT == SSMAP_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
     if constexpr (ACT == SSMAP_ACT_GELU) {
-        if constexpr (FINE) return half_erfc<true>(-0.70710678118654752f * z) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+        // the second term's limit is 0 where z may be infinite
+        if constexpr (FINE) {
+            const float bell = expf(-0.5f * z * z);
+            return half_erfc<true>(-0.70710678118654752f * z) + (bell > 0.0f ? z * 0.39894228040143268f * bell : 0.0f);
+        }
         // the formula of half_erfc at z / sqrt 2: its exponential is the bell
         const float a = fabsf(z), t = __builtin_amdgcn_rcpf(1.0f + kErfcAt * 0.70710678118654752f * a);
         const float bell = __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);
         const float tail = bell * erfc_ratio(t);
-        return (z < 0.0f ? tail : 1.0f - tail) + z * 0.39894228040143268f * bell;
+        return (z < 0.0f ? tail : 1.0f - tail) + (bell > 0.0f ? z * 0.39894228040143268f * bell : 0.0f);
     }
     if constexpr (ACT == SSMAP_ACT_GELU_TANH) {
         // q = (1 + tanh u) / 2; its slope in u is 2 q (1 - q), which is 0 where z may be infinite

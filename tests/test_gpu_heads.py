@@ -857,6 +857,27 @@ def test_linear_grad_of_a_single_class_whose_weight_is_a_turned_column():
     assert torch.equal(got.x, dy.transpose(1, 2) * w.float())
 
 
+@pytest.mark.parametrize("act", ACTS[1:])
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+def test_slope_where_pre_is_infinite(dtype, act):
+    """fp16 keeps a value beyond 65504 as infinity for the backward pass, beside a finite float32 result: its slope is
+    the limit, 1 or 0.  NaN stays NaN where the slope is computed from the value."""
+    big = {torch.float16: 300.0, torch.bfloat16: 1e4, torch.float32: 1e4}[dtype]
+    x = torch.tensor([[big, 1.0], [-big, 1.0], [0.5, 0.25]], dtype=dtype, device="cuda")
+    w = torch.tensor([[big, 0.0], [0.0, 1.0]], dtype=dtype, device="cuda")
+    y, pre = ssa.linear(x, w, activation=act, out_dtype=torch.float32, keep_pre=True)
+    assert torch.isfinite(y).all() and (dtype != torch.float16 or torch.isinf(pre[:2, 0]).all())
+    if dtype != torch.float16:
+        pre[0, 0], pre[1, 0] = math.inf, -math.inf
+    g = torch.tensor([[2.0, 0.0]] * 3, device="cuda")
+    got = ssa.linear_grad(g, x, w, activation=act, pre=pre)
+    assert got.x[0].tolist() == [2 * float(w[0, 0]), 0.0] and got.x[1].tolist() == [0.0, 0.0]
+    assert torch.isfinite(got.x).all() and torch.isfinite(got.weight).all() and torch.isfinite(got.bias).all()
+    pre[2, 0] = math.nan
+    if act != "relu":
+        assert torch.isnan(ssa.linear_grad(g, x, w, activation=act, pre=pre).x[2, 0])
+
+
 # ------------------------------------------------------------------ together, streams, graphs, the engine
 
 def test_a_training_step_of_a_head():
