@@ -8,7 +8,7 @@
 Each is one call of the C ABI on the current stream: it allocates its answers and a workspace with torch,
 enqueues its kernels and returns.  Nothing is kept between calls, so a call can be captured into a graph.
 The backward passes are functions of their own, not recorded by autograd: tensors that require a gradient
-are refused while autograd records.  There is no CPU fallback.
+are refused while autograd records, tensors with a tangent (forward mode) always.  There is no CPU fallback.
 
 The gradient of a log probability with respect to the temperature T needs no pass over the logits: it is
 -(log_prob + entropy) / T, which is what calibrating T on labelled frames descends along.
@@ -19,6 +19,7 @@ import ctypes as C
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _capi
 
@@ -44,8 +45,13 @@ class LinearGrads(NamedTuple):
     bias: Optional[torch.Tensor]
 
 
+def _tangent(t):
+    """Whether forward-mode differentiation follows t (no_grad does not stop it)."""
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
 def _gpu(device, **tensors):
-    """Every tensor lies on `device`, a GPU, and autograd would not record it."""
+    """Every tensor lies on `device`, a GPU, and neither mode of autograd would record it."""
     if device.type != "cuda":
         raise ValueError(f"expected tensors on a GPU, got {device}: the head operators have no CPU fallback")
     grad = torch.is_grad_enabled()
@@ -57,6 +63,9 @@ def _gpu(device, **tensors):
         if grad and t.requires_grad:
             raise RuntimeError(f"{name} requires a gradient, which autograd does not record here: call under "
                                "torch.no_grad() and use log_probs_grad / linear_grad for the backward pass")
+        if _tangent(t):
+            raise RuntimeError(f"{name} carries a tangent, which forward-mode differentiation does not get through here: "
+                               "pass its primal and use log_probs_grad / linear_grad")
 
 
 def _shape(name, t, dtype, shape):

@@ -1024,3 +1024,20 @@ def test_recorded_tensors_are_refused():
         ssa.log_probs(x.detach(), ids.cpu())
     with pytest.raises(ssa._capi.EngineError, match="temperature"):
         ssa.log_probs(x.detach(), ids, temperature=0.0)
+
+
+def test_tensors_with_a_tangent_are_refused():
+    """Forward mode would lose the derivative without a word, under no_grad as well."""
+    from torch.autograd import forward_ad
+    x, w = torch.randn((3, 5), device="cuda"), torch.randn((4, 5), device="cuda")
+    ids, y = torch.zeros(3, dtype=torch.int64, device="cuda"), torch.randn((3, 4), device="cuda")
+    s = ssa.log_probs(x, ids)
+    with forward_ad.dual_level(), torch.no_grad():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for name, call in (("logits", lambda t: ssa.log_probs(t, ids)), ("logits", lambda t: ssa.log_probs_grad(t, ids, s)),
+                           ("x", lambda t: ssa.linear(t, w)), ("x", lambda t: ssa.linear_grad(y, t, w))):
+            with pytest.raises(RuntimeError, match=name + " carries a tangent"):
+                call(dual)
+            call(x)
+        with pytest.raises(RuntimeError, match="residual carries a tangent"):
+            ssa.linear(x, w, residual=forward_ad.make_dual(y, torch.ones_like(y)))

@@ -174,3 +174,14 @@ def test_the_dense_axis_of_an_operand_is_not_read_from_its_strides():
     one = dict(layout=1, batch=16, rows=307200, inner=256, outer=1, g_batch_stride=307200, g_inner_stride=307200,
                x_batch_stride=307200 * 256, x_row_stride=256, g_x=16)
     assert _grad_workspace(**one, w_row_stride=1) == _grad_workspace(**one, w_row_stride=256) == 0
+
+
+def test_tangents_are_seen():
+    from torch.autograd import forward_ad
+    t = torch.ones(3)
+    assert not heads._tangent(t)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(t, torch.ones(3))
+        assert heads._tangent(dual) and not heads._tangent(t)
+        with torch.no_grad():
+            assert heads._tangent(dual) and not heads._tangent(forward_ad.unpack_dual(dual).primal)
