@@ -66,6 +66,8 @@ def _gpu(device, **tensors):
         if _tangent(t):
             raise RuntimeError(f"{name} carries a tangent, which forward-mode differentiation does not get through here: "
                                "pass its primal and use log_probs_grad / linear_grad")
+        if t.is_neg():   # a lazy view, as of a conjugate's imaginary part: memory holds the opposite values
+            raise ValueError(f"{name} is a view that negates when it is read; pass {name}.resolve_neg()")
 
 
 def _shape(name, t, dtype, shape):

@@ -1041,3 +1041,17 @@ def test_tensors_with_a_tangent_are_refused():
             call(x)
         with pytest.raises(RuntimeError, match="residual carries a tangent"):
             ssa.linear(x, w, residual=forward_ad.make_dual(y, torch.ones_like(y)))
+
+
+def test_views_that_negate_are_refused():
+    """As the imaginary part of a lazy conjugate is one: memory holds the opposite of its values."""
+    neg = torch._neg_view(torch.randn((3, 4), device="cuda"))
+    assert neg.is_neg() and torch.randn((3, 8), device="cuda").view(torch.complex64).conj().imag[:, :1].is_neg()
+    x, w, ids = torch.ones((3, 5), device="cuda"), torch.ones((4, 5), device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    for name, call in (("logits", lambda t: ssa.log_probs(t, ids)), ("grad_top", lambda t: ssa.log_probs_grad(w.t()[:3].contiguous(), ids, s, grad_top=t)),
+                       ("x", lambda t: ssa.linear(t, w[:, :4])), ("residual", lambda t: ssa.linear(x, w, residual=t)),
+                       ("grad", lambda t: ssa.linear_grad(t, x, w))):
+        s = ssa.log_probs(torch.ones((3, 4), device="cuda"), ids, top=4)
+        with pytest.raises(ValueError, match=name + " is a view that negates"):
+            call(neg)
+        call(neg.resolve_neg())
