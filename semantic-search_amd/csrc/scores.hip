@@ -68,15 +68,18 @@ struct Said {
     float log_prob, entropy, row_max, log_sum, log2_s;
     bool bad;
 };
-__device__ __forceinline__ Said say(const Shape &s, float m, float sum, float wsum, int64_t id, float xid) {
+__device__ __forceinline__ Said say(const Shape &s, float m, float sum, float wsum, bool ignored, bool inside, float xid) {
     const float nan = __builtin_nanf("");
     const bool bad = !(sum == sum), none = m == -INFINITY && !bad;
     const float log2_s = __log2f(sum);
     float given = (xid - m) * s.inv_t - kLn2 * log2_s;
     if (none) given = -INFINITY;
-    if (bad || id < 0 || id >= s.classes) given = nan;
-    if (id == s.ignore_id) given = 0.0f;
+    if (bad || !inside) given = nan;
+    if (ignored) given = 0.0f;
     return {given, bad ? nan : none ? 0.0f : kLn2 * (log2_s - wsum / sum), m, bad ? nan : none ? -INFINITY : kLn2 * log2_s, log2_s, bad};
+}
+__device__ __forceinline__ Said say(const Shape &s, float m, float sum, float wsum, int64_t id, float xid) {
+    return say(s, m, sum, wsum, id == s.ignore_id, id >= 0 && id < s.classes, xid);
 }
 __device__ __forceinline__ void put(const Out &o, int64_t pos, const Said &w) {
     o.log_prob[pos] = w.log_prob;
@@ -517,31 +520,42 @@ __device__ __forceinline__ void insert(float (&v)[K], int32_t (&i)[K], float x, 
     v[0] = above[0] ? x : v[0];
 }
 
+// sum += v, with what the addition rounds off taken along: sum - off is the sum.
+__device__ __forceinline__ void add_aside(float &sum, float &off, float v) {
+    const float y = v - off, to = sum + y;
+    off = (to - sum) - y;
+    sum = to;
+}
+
 constexpr int kPlaneClasses = 8;   // classes a plane kernel holds in flight
 
-// Planes: a thread walks the classes of PX neighbouring positions once, kPlaneClasses at a time: their
-// maximum first, so the running sums are rescaled once per step and not once per class.  K >= s.top.  Bound
-// by memory: 16 x 40 x 480 x 640 float32 with three alternatives takes 210 us, 4.7 TB/s (fetching the given
-// class afterwards and storing position by position 368 us).
+// Planes: a thread walks the classes of PX neighbouring positions once, kPlaneClasses at a time, whatever their number.
+// So that many classes cost no bits, each step's terms are summed by themselves and added to the running sums with
+// what the additions round off kept aside (true value: sum - sum_off); and the sums are rescaled only where a logit
+// exceeds their reference by more than a factor of two in its exponential, so that what a rescaling rounds fades by
+// half with the next.  K >= s.top.  Bound by memory: 16 x 40 x 480 x 640 float32 with three alternatives takes
+// 207 us, 4.8 TB/s (fetching the given class afterwards and storing position by position 368 us).
+// With five alternatives the registers stand at the border of five waves a SIMD (96): asked for, 250 and 301 us in
+// float32 and 16 bits; left to the compiler, which takes 97, 256 and 344.
 template <int DT, int PX, int K>
-__global__ __launch_bounds__(kThreads) void k_scores_planes(Shape s, const elem_t<DT> *logits, const void *ids, Out o) {
+__global__ __launch_bounds__(kThreads, K == 5 ? 5 : 1) void k_scores_planes(Shape s, const elem_t<DT> *logits, const void *ids, Out o) {
     const int64_t groups = (s.rows + PX - 1) / PX;
     const int64_t at = blockIdx.x * (int64_t)kThreads + threadIdx.x;
     if (at >= s.batch * groups) return;
     const int64_t b = at / groups, r0 = at % groups * PX;
     const bool full = r0 + PX <= s.rows;
     const elem_t<DT> *base = logits + b * s.batch_stride + r0;
-    float m[PX], sum[PX], wsum[PX], xid[PX], tv[PX][K ? K : 1];
-    int32_t ti[PX][K ? K : 1], id32[PX];
-    int64_t id[PX];
+    float m[PX], ref[PX], sum[PX], wsum[PX], sum_off[PX], wsum_off[PX], xid[PX], tv[PX][K ? K : 1];
+    int32_t ti[PX][K ? K : 1], id[PX];   // id: a class, kIgnored or kOutside
+    constexpr int32_t kIgnored = -1, kOutside = -2;
 #pragma unroll
     for (int q = 0; q < PX; ++q) {
         // the given class is picked up on the way: fetched afterwards, its line would come from memory again
-        id[q] = load_id(s, ids, b, r0 + q < s.rows ? r0 + q : r0);
-        id32[q] = id[q] >= 0 && id[q] < s.classes ? (int32_t)id[q] : -1;
+        const int64_t want = load_id(s, ids, b, r0 + q < s.rows ? r0 + q : r0);
+        id[q] = want == s.ignore_id ? kIgnored : want >= 0 && want < s.classes ? (int32_t)want : kOutside;
         xid[q] = 0.0f;
-        m[q] = -INFINITY;
-        sum[q] = wsum[q] = 0.0f;
+        m[q] = ref[q] = -INFINITY;
+        sum[q] = wsum[q] = sum_off[q] = wsum_off[q] = 0.0f;
 #pragma unroll
         for (int k = 0; k < K; ++k) tv[q][k] = -INFINITY, ti[q][k] = kNoId;
     }
@@ -561,27 +575,42 @@ __global__ __launch_bounds__(kThreads) void k_scores_planes(Shape s, const elem_
         }
 #pragma unroll
         for (int q = 0; q < PX; ++q) {
-            float mn = m[q];
+            float mn = x[0][q];
 #pragma unroll
-            for (int u = 0; u < kPlaneClasses; ++u) mn = fmaxf(mn, x[u][q]);
-            const float ms = mn == -INFINITY ? 0.0f : mn;
-            const float d = fmaxf((m[q] - ms) * s.scale, kTiny), a = __builtin_amdgcn_exp2f(d);
+            for (int u = 1; u < kPlaneClasses; ++u) mn = fmaxf(mn, x[u][q]);
+            if constexpr (K == 0) m[q] = fmaxf(m[q], mn);
+            const float was = ref[q];
+            if ((mn - was) * s.scale > 1.0f) ref[q] = mn;   // also the first maximum: -inf is in front of it
+            const float ms = ref[q] == -INFINITY ? 0.0f : ref[q];
+            const float d = fmaxf((was - ms) * s.scale, kTiny), a = __builtin_amdgcn_exp2f(d);   // 0 and 1 where it stays
             wsum[q] = a * (wsum[q] + sum[q] * d);
+            wsum_off[q] = a * (wsum_off[q] + sum_off[q] * d);
             sum[q] *= a;
-            m[q] = mn;
+            sum_off[q] *= a;
+            float part = 0.0f, wpart = 0.0f;
 #pragma unroll
             for (int u = 0; u < kPlaneClasses; ++u) {
                 const float t = (x[u][q] - ms) * s.scale, e = __builtin_amdgcn_exp2f(t);
-                sum[q] += e;
-                wsum[q] += e * fmaxf(t, kTiny);
-                xid[q] = id32[q] == (int32_t)(c0 + u) ? x[u][q] : xid[q];
+                part += e;
+                wpart += e * fmaxf(t, kTiny);
+                xid[q] = id[q] == (int32_t)(c0 + u) ? x[u][q] : xid[q];
                 if constexpr (K > 0) insert<K>(tv[q], ti[q], x[u][q], (int32_t)(c0 + u));
             }
+            add_aside(sum[q], sum_off[q], part);
+            add_aside(wsum[q], wsum_off[q], wpart);
         }
+    }
+#pragma unroll
+    for (int q = 0; q < PX; ++q) {   // relative to the maximum, which is at most a factor of two away
+        if constexpr (K > 0) m[q] = tv[q][0];
+        const float d = ref[q] == m[q] ? 0.0f : (ref[q] - m[q]) * s.scale, a = __builtin_amdgcn_exp2f(d);
+        sum[q] -= sum_off[q];
+        wsum[q] = a * (wsum[q] - wsum_off[q] + sum[q] * d);
+        sum[q] *= a;
     }
     Said said[PX];
 #pragma unroll
-    for (int q = 0; q < PX; ++q) said[q] = say(s, m[q], sum[q], wsum[q], id[q], xid[q]);
+    for (int q = 0; q < PX; ++q) said[q] = say(s, m[q], sum[q], wsum[q], id[q] == kIgnored, id[q] != kOutside, xid[q]);
     const auto put_row = [&](auto *to, auto value) {   // PX neighbours of one output plane
         using V = decltype(value(0));
         V v[PX];

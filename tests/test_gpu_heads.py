@@ -151,6 +151,30 @@ def test_planes(E, V, hw, top, dtype):
     check_scores(flat, plain_scores(x.movedim(1, -1).reshape(-1, V), ids.reshape(-1), float(np.float32(3.2)), top), V)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("V,top", [(5003, 2), (131072, 0)])
+def test_planes_of_many_classes(V, top, dtype):
+    """A vocabulary in planes: one thread sums all classes of a position, to no more roundings than few would cost.
+    Steps of eight classes are summed (8 roundings) and added with what the additions lose; a rescaling's three roundings
+    fade by half with the next; a term has five."""
+    g = gen(V)
+    at = torch.arange(V).float()
+    rows = [torch.randn(V, generator=g) * 2, torch.full((V,), -1.1), at / V, -at / V, at * (200.0 / V), (at % 97) / 97 - 0.3, torch.full((V,), 0.7)]
+    rows[1][0] = 0.0
+    x = torch.stack(rows).to(dtype)
+    ids = torch.tensor([0, 5, V - 1, V // 2, V - 1, 17, V])
+    T = 0.9
+    got = ssa.log_probs(x.t().contiguous()[None].cuda(), ids[None].cuda(), dim=1, top=top, temperature=T)
+    want = plain_scores(x, ids, float(np.float32(T)), top)
+    ls, H = want["log_sum"], want["entropy"]
+    base = U * (32 + 4 * ls.abs() + 4 * H)
+    close("log_sum", got.log_sum[0], ls, base)
+    close("log_prob", got.log_prob[0], want["log_prob"], base + 8 * U * want["log_prob"].nan_to_num(0).abs())
+    close("entropy", got.entropy[0], H, U * (32 * (1 + H) + 8 * H + 4 * want["t2"]) + base)
+    assert torch.equal(got.top_ids[0].t().cpu().long(), want["top_ids"])
+    assert got.row_max[0].cpu().double().equal(x.double().max(1).values)
+
+
 def special_rows(V, dtype, seed):
     """Rows with masks, ties, infinities and the type's extremes, and ids to match."""
     g = gen(seed)
@@ -215,6 +239,18 @@ def test_special_planes(dtype):
     got = ssa.log_probs(x.t().contiguous()[None].cuda(), ids[None].cuda(), dim=1, top=5)
     flat = got._replace(top_ids=got.top_ids[0].t(), top_log_prob=got.top_log_prob[0].t())
     check_scores(flat, plain_scores(x, ids, 1.0, 5), 40)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("V,top", [(40, 0), (40, 1), (40, 3), (41, 9), (700, 20), (3, 2), (1, 0)])
+def test_special_planes_with_any_number_of_alternatives(V, top, dtype):
+    x, ids = special_rows(V, dtype, V + top)
+    got = ssa.log_probs(x.t().contiguous()[None].cuda(), ids[None].cuda(), dim=1, top=top)
+    flat = got._replace(top_ids=got.top_ids[0].t(), top_log_prob=got.top_log_prob[0].t())
+    check_scores(flat, plain_scores(x, ids, 1.0, top), V)
+    # an ignored id may be a class
+    got = ssa.log_probs(x.t().contiguous()[None].cuda(), ids[None].cuda(), dim=1, top=top, ignore_id=0)
+    check_scores(got._replace(top_ids=got.top_ids[0].t(), top_log_prob=got.top_log_prob[0].t()), plain_scores(x, ids, 1.0, top, ignore=0), V)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
