@@ -44,18 +44,18 @@ __device__ __forceinline__ f32x4 mma_chunk(i32x4 j, i32x4 i, f32x4 acc) {
 
 constexpr uint32_t kNowhere = 0xFFFFFFF0u;   // a buffer offset behind every descriptor's end: reads as zero
 
-// One side of a tile: R rows (or columns) of it, C chunks of the sum's direction a stage, NT threads.
-template <int DT, bool KC, int R, int C, int NT>
+// One side of a tile: R rows (or columns) of it, eight chunks of the sum's direction a stage, NT threads.
+template <int DT, bool KC, int R, int NT>
 struct Side {
-    static constexpr int SIZE = head_dtype_size(DT), E = 16 / SIZE, KB = C * E;   // values a chunk, a stage
+    static constexpr int C = 8, SIZE = head_dtype_size(DT), E = 16 / SIZE, KB = C * E;   // chunks a stage; values a chunk, a stage
     static constexpr int PER = R * C / NT, ROW = R / E;                           // chunks a thread; a row (not KC)
     static constexpr int BYTES = R * C * 16;
-    static_assert((C == 4 || C == 8) && R * C % NT == 0 && (KC || ROW >= 8), "tile shape");
+    static_assert(R * C % NT == 0 && (KC || ROW >= 8), "tile shape");
 
     static __device__ __forceinline__ int swizzle(int k) { return DT == SSMAP_F32 ? ((k >> 2) & 3) << 2 : (k & 3) << 1; }
 
     // KC: 128 bytes of consecutive slots hold eight rows' chunks of one c
-    static __device__ __forceinline__ int turn(int row) { return C == 8 ? row & 7 : (row >> 1) & 3; }
+    static __device__ __forceinline__ int turn(int row) { return row & 7; }
 
     // chunk of slot s: its row (KC) or sum index (not KC), and its place there
     static __device__ __forceinline__ void place(int s, int &line, int &c) {
@@ -252,13 +252,13 @@ __device__ __forceinline__ void finish_at(const Product &p, int64_t e, int64_t m
     finish<WHOLE, DT, OT, N, PAST>(p, (e * p.M + m) * p.N + n, left, z, bias, res);
 }
 
-// BI x BJ results a block, WI x WJ waves, stages of C chunks in NBUF buffers.  DIRECT: both sides go straight to
-// LDS (see Side::fetch), NBUF - 1 stages ahead; otherwise through registers, one stage ahead.
-template <int DT, int OT, bool IK, bool JK, int BI, int BJ, int WI, int WJ, int C, int NBUF, bool DIRECT>
+// BI x BJ results a block, WI x WJ waves, stages in NBUF buffers.  DIRECT: both sides go straight to LDS (see
+// Side::fetch), NBUF - 1 stages ahead; otherwise through registers, one stage ahead.
+template <int DT, int OT, bool IK, bool JK, int BI, int BJ, int WI, int WJ, int NBUF, bool DIRECT>
 __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
     constexpr int NT = WI * WJ * 64, TI = BI / WI / 16, TJ = BJ / WJ / 16, SIZE = head_dtype_size(DT);
-    using I = Side<DT, IK, BI, C, NT>;
-    using J = Side<DT, JK, BJ, C, NT>;
+    using I = Side<DT, IK, BI, NT>;
+    using J = Side<DT, JK, BJ, NT>;
     constexpr int PITCH = TJ * 16 + 4;                 // floats a row while results are turned: four off, for the banks
     constexpr int HI = TI > 4 ? TI / 2 : TI;           // rows of 16 turned at once
     constexpr int LINE = TJ * 16 / 8, ROWS = 64 / LINE;   // lanes a row, rows at once
@@ -280,8 +280,7 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
         const int64_t in_band = tile % (BAND * tiles_n);
         const int64_t i0 = (band * BAND + in_band % rows_in) * BI, j0 = in_band / rows_in * BJ;
         const int rows_i = (int)(p.M - i0 < BI ? p.M - i0 : BI), rows_j = (int)(p.N - j0 < BJ ? p.N - j0 : BJ);
-        const int64_t part = p.part_steps * (8 / C);   // planned in stages of eight chunks
-        const int64_t first = split * part, last = first + part < all_steps ? first + part : all_steps;
+        const int64_t first = split * p.part_steps, last = first + p.part_steps < all_steps ? first + p.part_steps : all_steps;
         const int64_t ld_i = (IK ? p.a_m : p.a_k) * SIZE, ld_j = (JK ? p.b_n : p.b_k) * SIZE;
         const int64_t step_i = (IK ? 1 : p.a_k) * (int64_t)(I::KB * SIZE), step_j = (JK ? 1 : p.b_k) * (int64_t)(I::KB * SIZE);
         const char *pa = static_cast<const char *>(p.a) + (e * p.a_out + i0 * p.a_m) * SIZE;
@@ -362,7 +361,7 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
             // first waves send for it in turn 4t, the second ones in turn 4t + 1, each behind its reads (in front
             // of them or of the matrix instructions the queue of loads held those up: 937 against 896 us at
             // 8192^3), and all have waited for it at the end of turn 4t + 3.
-            static_assert(DIRECT && C == 8 && NBUF == 2, "two turns a stage");
+            static_assert(DIRECT && NBUF == 2, "two turns a stage");
             const bool late = wave >= 4;
             const auto turn_ends = [&] {
                 __builtin_amdgcn_sched_barrier(0);
@@ -429,10 +428,10 @@ __global__ __launch_bounds__(WI *WJ * 64) void k_tiles(Product p) {
                 // the reads here: two blocks a CU keep each other busy, and behind the reads they come late (626).
                 i32x4 gi[TI], gj[TJ];
                 read(buf, 0, fi, fj);
-                if constexpr (C == 8) read(buf, 1, gi, gj);
+                read(buf, 1, gi, gj);
                 __builtin_amdgcn_sched_barrier(0);
                 multiply(fi, fj);
-                if constexpr (C == 8) multiply(gi, gj);
+                multiply(gi, gj);
                 if (more) keep(next);
                 buf = buf + 1 == NBUF ? 0 : buf + 1;
             }
@@ -611,9 +610,9 @@ __global__ __launch_bounds__(kFewWaves * 64) void k_few_rows(Product p) {
             const int left = (int)(p.N - n < 4 ? p.N - n : 4);
             float z[4] = {v[0], v[1], v[2], v[3]};
             if (m < p.M && left > 0) {
-            if (left == 4) finish_at<true, DT, OT, 4>(p, e, m, n, 4, z);
-            else finish_at<false, DT, OT, 4>(p, e, m, n, left, z);
-        }
+                if (left == 4) finish_at<true, DT, OT, 4>(p, e, m, n, 4, z);
+                else finish_at<false, DT, OT, 4>(p, e, m, n, left, z);
+            }
         }
     }
 }
@@ -683,26 +682,26 @@ __global__ __launch_bounds__(256) void k_head(Product p, int pitch) {
 
 template <int DT, int OT, bool IK, bool JK>
 void launch_tiles(const Product &p, hipStream_t st) {
-    const auto go = [&](auto bi, auto bj, auto wi, auto wj, auto c, auto nbuf, auto d) {
+    const auto go = [&](auto bi, auto bj, auto wi, auto wj, auto nbuf, auto d) {
         const int64_t tiles = (p.M + bi.value - 1) / bi.value * ((p.N + bj.value - 1) / bj.value) * p.out_batches;
-        k_tiles<DT, OT, IK, JK, bi.value, bj.value, wi.value, wj.value, c.value, nbuf.value, d.value><<<blocks(tiles * p.splits), wi.value * wj.value * 64, 0, st>>>(p);
+        k_tiles<DT, OT, IK, JK, bi.value, bj.value, wi.value, wj.value, nbuf.value, d.value>
+            <<<blocks(tiles * p.splits), wi.value * wj.value * 64, 0, st>>>(p);
     };
     using std::integral_constant;
     const integral_constant<int, 1> one{};
     const integral_constant<int, 2> two{};
     const integral_constant<int, 4> four{};
-    const integral_constant<int, 8> eight{};
     const integral_constant<int, 64> narrow{};
     const integral_constant<int, 128> mid{};
     const integral_constant<int, 256> big{};
     if constexpr (DT != SSMAP_F32)
-        if (p.shape == kTileBig) return go(big, big, two, four, eight, two, std::true_type{});
-    if (p.shape == kTileMid) go(mid, mid, two, two, eight, two, std::true_type{});
-    else if (p.shape == kTileLow) go(narrow, big, one, four, eight, two, std::true_type{});
-    else if (p.shape == kTileTall) go(big, narrow, four, one, eight, two, std::true_type{});
-    else if (p.shape == kTileSmall) go(narrow, narrow, two, two, eight, four, std::true_type{});
-    else if (p.shape == kTileSmallAny) go(narrow, narrow, two, two, eight, two, std::false_type{});
-    else go(mid, mid, two, two, eight, two, std::false_type{});
+        if (p.shape == kTileBig) return go(big, big, two, four, two, std::true_type{});
+    if (p.shape == kTileMid) go(mid, mid, two, two, two, std::true_type{});
+    else if (p.shape == kTileLow) go(narrow, big, one, four, two, std::true_type{});
+    else if (p.shape == kTileTall) go(big, narrow, four, one, two, std::true_type{});
+    else if (p.shape == kTileSmall) go(narrow, narrow, two, two, four, std::true_type{});
+    else if (p.shape == kTileSmallAny) go(narrow, narrow, two, two, two, std::false_type{});
+    else go(mid, mid, two, two, two, std::false_type{});
 }
 
 // Lines of `dense` values to lines of `pitch` ones (a multiple of 16 bytes), filled up with zeros.
