@@ -278,9 +278,10 @@ int ssmap_path_paint(ssmap_engine *eng, void *stream);
  *
  * They belong to no engine: the caller passes device pointers, shapes and strides (in elements), a
  * stream of the current device and, where ssmap_*_workspace() asks for one, a workspace that is used by
- * this call alone until its work on the stream is done (at a multiple of 16 bytes).  Strides are not negative.  Nothing is allocated, nothing waits, nothing is
- * kept between calls, so a call may be captured into a graph and replayed.  No counterpart in the
- * reference, whose networks end in library calls (infer.py:95-118, 301-327 hold what follows them).
+ * this call alone until its work on the stream is done (at a multiple of 16 bytes).  Strides are not
+ * negative.  Nothing is allocated, nothing waits, nothing is kept between calls, so a call may be captured
+ * into a graph and replayed.  No counterpart in the reference, whose networks end in library calls
+ * (infer.py:95-118, 301-327 hold what follows them).
  *
  * Two layouts.  SSMAP_ROWS: the classes lie last, [batch][rows][classes], as a language model leaves its
  * logits.  SSMAP_PLANES: one plane per class, [batch][classes][rows], as a segmentation head leaves them
@@ -333,9 +334,9 @@ int ssmap_log_probs(const ssmap_log_probs_args *args, void *stream);
  *   d / d logit_j = ( g_l ([j = id] - p_j) + sum_k g_top_k ([j = top_id_k] - p_j)
  *                     - g_e p_j (log p_j + entropy) ) / temperature.
  * row_max, log_sum, entropy and top_ids are ssmap_log_probs' answers for the same logits.  Ignored ids
- * and alternatives with an id outside [0, classes) give nothing; no alternative stands twice in a position.  A position whose classes are all masked has the gradient 0;
- * one without a distribution, or with an id outside [0, classes) and a g_log_prob given, NaN.  A
- * gradient that is NULL counts as 0. */
+ * and alternatives with an id outside [0, classes) give nothing; no alternative stands twice in a position.
+ * A position whose classes are all masked has the gradient 0; one without a distribution, or with an id
+ * outside [0, classes) and a g_log_prob given, NaN.  A gradient that is NULL counts as 0. */
 typedef struct ssmap_log_probs_grad_args {
     int32_t dtype, layout;
     int64_t batch, rows, classes;

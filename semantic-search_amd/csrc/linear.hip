@@ -36,6 +36,16 @@ inline bool direct_side(const void *p, int64_t line, int64_t out, int64_t sum, i
 constexpr int kDzRows = 128;       // rows: positions a block sums; 8 threads down, 32 packs of 8 outputs across
 constexpr int kDzPlane = 16384;    // planes: positions a block sums
 
+struct Dz {
+    int64_t batch, rows, outer;
+    int64_t g_batch, g_line;           // strides of g
+    int64_t line;                      // values a line of dz takes, zeros behind the dense ones
+    int64_t rest;                      // what dz's roundings left lies that many values behind it; 0: not kept
+    int32_t act;
+    const float *scale;                // what dz is multiplied by, or NULL
+    float *sums;                       // for the bias's gradient, or NULL
+};
+
 // Eight neighbours, of which `left` exist; WHOLE: all, which the caller knows for its whole wave.
 template <bool WHOLE, int T>
 __device__ __forceinline__ void load8(const elem_t<T> *p, int left, float (&v)[8]) {
@@ -50,15 +60,16 @@ __device__ __forceinline__ void load8(const elem_t<T> *p, int left, float (&v)[8
     }
 }
 template <bool WHOLE, int DT, int OT>
-__device__ __forceinline__ void dz_pack(const elem_t<OT> *g, const elem_t<DT> *pre, elem_t<DT> *dz, int64_t rest, float by, int left, int room, int act, float (&sum)[8]) {   // room: of dz's line, zeros included
+__device__ __forceinline__ void dz_pack(const Dz &a, float by, const elem_t<OT> *g, const elem_t<DT> *pre, elem_t<DT> *dz, int left, int room,
+                                        float (&sum)[8]) {   // room: of dz's line, zeros included
     float v[8];
     load8<WHOLE, OT>(g, left, v);
     if (pre) {
         float z[8];
         load8<WHOLE, DT>(pre, left, z);
-        with_activation(act, [&](auto a) {
+        with_activation(a.act, [&](auto act) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] *= slope<a.value, DT == SSMAP_F32>(z[e]);
+            for (int e = 0; e < 8; ++e) v[e] *= slope<act.value, DT == SSMAP_F32>(z[e]);
         });
     }
 #pragma unroll
@@ -74,7 +85,7 @@ __device__ __forceinline__ void dz_pack(const elem_t<OT> *g, const elem_t<DT> *p
                 if (e < room) to[e] = e < left ? w[e] : Elem<DT>::put(0.0f);
         }
     };
-    if (DT == SSMAP_F32 || !rest) {
+    if (DT == SSMAP_F32 || !a.rest) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = Elem<DT>::put(v[e]);
         return keep(dz);
@@ -90,13 +101,14 @@ __device__ __forceinline__ void dz_pack(const elem_t<OT> *g, const elem_t<DT> *p
     keep(dz);
 #pragma unroll
     for (int e = 0; e < 8; ++e) w[e] = Elem<DT>::put(v[e]);
-    keep(dz + rest);
+    keep(dz + a.rest);
 }
 
 // The largest finite |g| of each block's share: lines of `dense` values, `lines` a batch.
 constexpr int kPeaks = 1024;   // blocks at most
 template <int OT>
-__global__ __launch_bounds__(256) void k_peak(int64_t batch, int64_t lines, int64_t dense, const elem_t<OT> *g, int64_t g_batch, int64_t g_line, float *peaks) {
+__global__ __launch_bounds__(256) void k_peak(int64_t batch, int64_t lines, int64_t dense, const elem_t<OT> *g, int64_t g_batch, int64_t g_line,
+                                              float *peaks) {
     __shared__ float part[4];
     const int64_t per = (dense + 7) / 8, units = batch * lines * per;
     float peak = 0.0f;
@@ -131,29 +143,29 @@ __global__ __launch_bounds__(kPeaks) void k_scale(const float *peaks, int n, flo
     scale[1] = __builtin_bit_cast(float, (uint32_t)(127 - by) << 23);
 }
 
-// sums[batch * row chunks][outer]; `rest`: what the roundings left lies that many values behind, or 0
+// sums[batch * row chunks][outer]
 template <int DT, int OT>
-__global__ __launch_bounds__(256) void k_dz_rows(int64_t batch, int64_t rows, int64_t outer, const elem_t<OT> *g, int64_t g_batch, int64_t g_row,
-                                                 const elem_t<DT> *pre, int act, elem_t<DT> *dz, int64_t dz_line, int64_t rest, const float *scale, float *sums) {
-    const float by = scale ? *scale : 1.0f;
+__global__ __launch_bounds__(256) void k_dz_rows(Dz a, const elem_t<OT> *g, const elem_t<DT> *pre, elem_t<DT> *dz) {
     __shared__ float part[8][256];
+    const float by = a.scale ? *a.scale : 1.0f;
     const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
-    const int64_t strips = (outer + 255) / 256, chunks = (rows + kDzRows - 1) / kDzRows;
-    for (int64_t unit = blockIdx.x; unit < strips * chunks * batch; unit += gridDim.x) {
+    const int64_t rows = a.rows, outer = a.outer, strips = (outer + 255) / 256, chunks = (rows + kDzRows - 1) / kDzRows;
+    for (int64_t unit = blockIdx.x; unit < strips * chunks * a.batch; unit += gridDim.x) {
         const int64_t n = unit % strips * 256 + tx * 8, bc = unit / strips, b = bc / chunks, r0 = bc % chunks * kDzRows;
-        const int left = (int)(outer - n < 8 ? outer - n : 8);
+        const int left = (int)(outer - n < 8 ? outer - n : 8), room = (int)(a.line - n < 8 ? a.line - n : 8);
         float sum[8] = {};
         const int64_t end = r0 + kDzRows < rows ? r0 + kDzRows : rows;
         const auto walk = [&](auto whole) {
 #pragma unroll 2
             for (int64_t r = r0 + ty; r < end; r += 8) {
                 const int64_t o = (b * rows + r) * outer + n;
-                dz_pack<whole.value, DT, OT>(g + b * g_batch + r * g_row + n, pre ? pre + o : nullptr, dz ? dz + (b * rows + r) * dz_line + n : nullptr, rest, by, left, (int)(dz_line - n < 8 ? dz_line - n : 8), act, sum);
+                dz_pack<whole.value, DT, OT>(a, by, g + b * a.g_batch + r * a.g_line + n, pre ? pre + o : nullptr,
+                                             dz ? dz + (b * rows + r) * a.line + n : nullptr, left, room, sum);
             }
         };
         if (unit % strips * 256 + 256 <= outer) walk(std::true_type{});
         else if (left > 0) walk(std::false_type{});
-        if (!sums) continue;
+        if (!a.sums) continue;
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < 8; ++e) part[ty][tx * 8 + e] = sum[e];
@@ -162,41 +174,40 @@ __global__ __launch_bounds__(256) void k_dz_rows(int64_t batch, int64_t rows, in
         float s = 0.0f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) s += part[k][threadIdx.x];
-        if (out < outer) sums[bc * outer + out] = s;
+        if (out < outer) a.sums[bc * outer + out] = s;
     }
 }
 
 // sums[batch * chunks][outer]
 template <int DT, int OT>
-__global__ __launch_bounds__(256) void k_dz_planes(int64_t batch, int64_t rows, int64_t outer, const elem_t<OT> *g, int64_t g_batch, int64_t g_plane,
-                                                   const elem_t<DT> *pre, int act, elem_t<DT> *dz, int64_t dz_line, int64_t rest, const float *scale, float *sums) {
-    const float by = scale ? *scale : 1.0f;
+__global__ __launch_bounds__(256) void k_dz_planes(Dz a, const elem_t<OT> *g, const elem_t<DT> *pre, elem_t<DT> *dz) {
     __shared__ float part[256];
-    const int64_t chunks = (rows + kDzPlane - 1) / kDzPlane;
-    for (int64_t unit = blockIdx.x; unit < chunks * outer * batch; unit += gridDim.x) {
+    const float by = a.scale ? *a.scale : 1.0f;
+    const int64_t rows = a.rows, outer = a.outer, chunks = (rows + kDzPlane - 1) / kDzPlane;
+    for (int64_t unit = blockIdx.x; unit < chunks * outer * a.batch; unit += gridDim.x) {
         const int64_t c = unit % chunks, bn = unit / chunks, b = bn / outer, n = bn % outer;
         float sum[8] = {};
         const int64_t end = (c + 1) * kDzPlane < rows ? (c + 1) * kDzPlane : rows;
-        const elem_t<OT> *gp = g + b * g_batch + n * g_plane;
+        const elem_t<OT> *gp = g + b * a.g_batch + n * a.g_line;
         const elem_t<DT> *zp = pre ? pre + bn * rows : nullptr;
-        elem_t<DT> *dp = dz ? dz + bn * dz_line : nullptr;
+        elem_t<DT> *dp = dz ? dz + bn * a.line : nullptr;
         int64_t r = c * kDzPlane;
 #pragma unroll 2
         for (; r + 2048 <= end; r += 2048) {
             const int64_t at = r + threadIdx.x * 8;
-            dz_pack<true, DT, OT>(gp + at, zp ? zp + at : nullptr, dp ? dp + at : nullptr, rest, by, 8, 8, act, sum);
+            dz_pack<true, DT, OT>(a, by, gp + at, zp ? zp + at : nullptr, dp ? dp + at : nullptr, 8, 8, sum);
         }
         const int64_t at = r + threadIdx.x * 8;
-        if (at < end) dz_pack<false, DT, OT>(gp + at, zp ? zp + at : nullptr, dp ? dp + at : nullptr, rest, by, (int)(end - at < 8 ? end - at : 8),
-                                           (int)(end < rows ? 8 : dz_line - at < 8 ? dz_line - at : 8), act, sum);
-        if (!sums) continue;
+        const int left = (int)(end - at < 8 ? end - at : 8), room = (int)(end < rows ? 8 : a.line - at < 8 ? a.line - at : 8);
+        if (at < end) dz_pack<false, DT, OT>(a, by, gp + at, zp ? zp + at : nullptr, dp ? dp + at : nullptr, left, room, sum);
+        if (!a.sums) continue;
         part[threadIdx.x] = ((sum[0] + sum[1]) + (sum[2] + sum[3])) + ((sum[4] + sum[5]) + (sum[6] + sum[7]));
         __syncthreads();
         for (int d = 128; d; d >>= 1) {
             if (threadIdx.x < d) part[threadIdx.x] += part[threadIdx.x + d];
             __syncthreads();
         }
-        if (!threadIdx.x) sums[(b * chunks + c) * outer + n] = part[0];
+        if (!threadIdx.x) a.sums[(b * chunks + c) * outer + n] = part[0];
         __syncthreads();
     }
 }
@@ -382,12 +393,12 @@ int ssmap_linear_grad(const ssmap_linear_grad_args *a, void *stream) {
             k_scale<<<1, kPeaks, 0, st>>>(scale + 2, (int)n, scale);
         }
         if (positions * a->outer && (dz || sums)) {
-            if (q.planes)
-                k_dz_planes<DT, OT><<<blocks(q.chunks * a->outer), 256, 0, st>>>(a->batch, a->rows, a->outer, g, a->g_batch_stride, a->g_inner_stride, pre, a->activation, dz, q.dz_line, q.dz_rest, scale, sums);
-            else
-                k_dz_rows<DT, OT><<<blocks(q.chunks * ((a->outer + 255) / 256)), 256, 0, st>>>(a->batch, a->rows, a->outer, g, a->g_batch_stride, a->g_inner_stride, pre, a->activation, dz, q.dz_line, q.dz_rest, scale, sums);
+            const Dz z{a->batch, a->rows, a->outer, a->g_batch_stride, a->g_inner_stride, q.dz_line, q.dz_rest, a->activation, scale, sums};
+            if (q.planes) k_dz_planes<DT, OT><<<blocks(q.chunks * a->outer), 256, 0, st>>>(z, g, pre, dz);
+            else k_dz_rows<DT, OT><<<blocks(q.chunks * ((a->outer + 255) / 256)), 256, 0, st>>>(z, g, pre, dz);
         }
-        if (a->g_bias && a->outer) k_bias_grad<DT><<<blocks((a->outer + 3) / 4), 256, 0, st>>>(q.chunks, a->outer, sums, static_cast<elem_t<DT> *>(a->g_bias));
+        if (a->g_bias && a->outer)
+            k_bias_grad<DT><<<blocks((a->outer + 3) / 4), 256, 0, st>>>(q.chunks, a->outer, sums, static_cast<elem_t<DT> *>(a->g_bias));
         if (a->g_x) launch_product<DT, DT>(q.x, st);
         if (a->g_w) launch_product<DT, DT>(q.w, st);
     });
@@ -414,8 +425,8 @@ int64_t ssmap::plan_product(Product &p, int dtype) {
     bool direct = direct_a && direct_b;
     const auto tiles = [&](int bi, int bj) { return (p.M + bi - 1) / bi * ((p.N + bj - 1) / bj) * p.out_batches; };
     const int64_t e = 16 / size;
-    if (p.M <= kHeadMost && ik && jk && p.sum_batches == 1 && p.a_out == 0 && p.K >= e && p.K % e == 0 && head_bytes(p, size) <= kHeadBytes &&
-        p.N * p.out_batches >= 16384) {
+    if (p.M <= kHeadMost && ik && jk && p.sum_batches == 1 && p.a_out == 0 && p.K >= e && p.K % e == 0 &&
+        head_bytes(p, size) <= kHeadBytes && p.N * p.out_batches >= 16384) {
         p.shape = kHead;
         return 0;
     }

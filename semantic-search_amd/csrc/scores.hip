@@ -303,7 +303,8 @@ struct Part {       // what a segment of a split row says, followed by `top` alt
 // caches, and only logits that reach it become candidates.  4096 x 32003 fp16 with five alternatives takes 62 us
 // (the bytes 51), 2048 x 131072 bf16 with twenty 110 us (104).
 template <int DT>
-__global__ __launch_bounds__(kThreads, 8) void k_scores_long(Shape s, const elem_t<DT> *logits, const void *ids, Out o, int splits, int64_t segment, char *parts, int64_t part_bytes) {
+__global__ __launch_bounds__(kThreads, 8) void k_scores_long(Shape s, const elem_t<DT> *logits, const void *ids, Out o, int splits,
+                                                             int64_t segment, char *parts, int64_t part_bytes) {
     constexpr int VEC = 16 / sizeof(elem_t<DT>), U = kLongPacks, STEP = kThreads * VEC;
     __shared__ Sums joint[kThreads / 64];
     __shared__ Key firsts[kThreads];
@@ -437,7 +438,8 @@ __global__ __launch_bounds__(kThreads, 8) void k_scores_long(Shape s, const elem
 // Joins the segments of a split row: one block per row, at most kThreads segments.  The `top` segments with
 // the best first alternatives hold all of the row's.
 template <int DT>
-__global__ __launch_bounds__(kThreads) void k_scores_join(Shape s, const elem_t<DT> *logits, const void *ids, Out o, int splits, const char *parts, int64_t part_bytes) {
+__global__ __launch_bounds__(kThreads) void k_scores_join(Shape s, const elem_t<DT> *logits, const void *ids, Out o, int splits, const char *parts,
+                                                          int64_t part_bytes) {
     __shared__ Sums joint[kThreads / 64];
     __shared__ Key firsts[kThreads], least;
     __shared__ Candidates cand;

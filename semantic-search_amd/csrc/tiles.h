@@ -732,15 +732,16 @@ __global__ __launch_bounds__(256) void k_pack(const elem_t<DT> *from, int64_t ba
 // Copies one operand (strides: dense across or along the sum; `blocks_in_sum` of it) behind p.parts and points at
 // the copy.
 template <int DT>
-void pack_side(const Product &p, int64_t at, bool kc, int64_t rows, int64_t blocks_in_sum, const void *&side, int64_t &row, int64_t &k, int64_t &out, int64_t &sum, hipStream_t st) {
+void pack_side(const Product &p, int64_t at, bool kc, int64_t rows, int64_t blocks_in_sum, const void *&side, int64_t &row, int64_t &k,
+               int64_t &out, int64_t &sum, hipStream_t st) {
     if (at < 0) return;
     constexpr int64_t E = 16 / sizeof(elem_t<DT>);
     const int64_t lines = kc ? rows : p.K, dense = kc ? p.K : rows, pitch = (dense + E - 1) / E * E;
     const int64_t batches = p.sum_batches > 1 ? blocks_in_sum : out ? p.out_batches : 1;
     elem_t<DT> *to = reinterpret_cast<elem_t<DT> *>(reinterpret_cast<char *>(p.parts) + at);
     const int64_t units = batches * lines * (pitch / E);
-    k_pack<DT><<<blocks((units + 255) / 256), 256, 0, st>>>(static_cast<const elem_t<DT> *>(side), p.sum_batches > 1 ? sum : out, kc ? row : k, batches, lines, dense,
-                                                            pitch, to);
+    k_pack<DT><<<blocks((units + 255) / 256), 256, 0, st>>>(static_cast<const elem_t<DT> *>(side), p.sum_batches > 1 ? sum : out,
+                                                            kc ? row : k, batches, lines, dense, pitch, to);
     side = to;
     (kc ? row : k) = pitch;
     if (out) out = lines * pitch;
