@@ -182,7 +182,8 @@ def log_probs(logits: torch.Tensor, ids: torch.Tensor, *, dim: int = -1, tempera
     Ties go to the lowest class.  An id equal to `ignore_id` has log probability 0, any other id outside
     [0, classes) NaN.  A logit of -inf masks its class; where fewer than `top` classes are left, the other
     alternatives have id -1 and log probability -inf; where none is, log_prob is -inf and the entropy 0.  A
-    position that holds a NaN or +inf has NaN for everything and ids -1.
+    position that holds a NaN or +inf has NaN for everything but row_max (the largest that is a number) and
+    an ignored id's 0, and ids -1.
     """
     dt = _dtype("logits", logits)
     top = int(top)
