@@ -357,8 +357,8 @@ int ssmap_log_probs_grad(const ssmap_log_probs_grad_args *args, void *stream);
 
 /* y = act(x w^T + bias) + residual.  x [batch][rows][inner], w [outer][inner]; y, residual and pre are
  * [batch][rows][outer] in rows, [batch][outer][rows] in planes.  Products of 16-bit values are summed in
- * 32 bits, in an order that the sizes alone decide; the sum is rounded once, to out_dtype.  `pre`, if
- * given, receives x w^T + bias (rounded to dtype), which ssmap_linear_grad needs where there is an
+ * 32 bits, in an order that sizes, strides and the pointers' alignment decide (an operand out of line takes
+ * another kernel); the sum is rounded once, to out_dtype.  `pre`, if given, receives x w^T + bias (rounded to dtype), which ssmap_linear_grad needs where there is an
  * activation. */
 typedef struct ssmap_linear_args {
     int32_t dtype;                     /* of x, w and pre */

@@ -489,7 +489,10 @@ __global__ __launch_bounds__(kThreads) void k_scores_join(Shape s, const elem_t<
 }
 
 // Segments of a long row: one where the rows alone fill the card (two blocks a CU), otherwise enough for
-// four, each at least one pack a thread.
+// four, each at least one pack a thread.  131072 bf16 classes with five alternatives, against half as many
+// blocks and twice as many: 32 rows 19.0 us, 16.1 and 26.3; 128 rows 22.9, 22.9 and 26.5; 256 rows 29.0 and whole
+// 32.5; 700 rows whole 45.1 and split 48.3.  Rows of a few thousand classes pay for the join: 511 x 5000 20.5 and
+// whole 13.4.
 struct Split {
     int splits;
     int64_t segment, part_bytes;
@@ -871,6 +874,8 @@ void launch_scores(const Shape &s, const ssmap_log_probs_args &a, hipStream_t st
         if (s.classes <= 48 * VEC) return brief(std::integral_constant<int, 16>{}, std::integral_constant<int, 3>{});
         if (s.classes <= 64 * VEC) return brief(std::integral_constant<int, 16>{}, std::integral_constant<int, 4>{});
     }
+    // 4096 x 600 bf16 takes 4.8 us here and 14.6 as long rows, 13.8 and 32.3 with five alternatives.  Twice the registers,
+    // for 2000 classes: 8.7 and 14.8, with alternatives 32.4 and 32.2, of 64 rows 15.8 and 10.8.
     if (s.classes <= 64 * VEC * NP) return brief(std::integral_constant<int, 64>{}, std::integral_constant<int, NP>{});
     const Split w = split_rows(s, DT);
     char *parts = static_cast<char *>(a.workspace);
