@@ -358,8 +358,8 @@ int ssmap_log_probs_grad(const ssmap_log_probs_grad_args *args, void *stream);
 /* y = act(x w^T + bias) + residual.  x [batch][rows][inner], w [outer][inner]; y, residual and pre are
  * [batch][rows][outer] in rows, [batch][outer][rows] in planes.  Products of 16-bit values are summed in
  * 32 bits, in an order that sizes, strides and the pointers' alignment decide (an operand out of line takes
- * another kernel); the sum is rounded once, to out_dtype.  `pre`, if given, receives x w^T + bias (rounded to dtype), which ssmap_linear_grad needs where there is an
- * activation. */
+ * another kernel); the sum is rounded once, to out_dtype.  `pre`, if given, receives x w^T + bias (rounded
+ * to dtype), which ssmap_linear_grad needs where there is an activation. */
 typedef struct ssmap_linear_args {
     int32_t dtype;                     /* of x, w and pre */
     int32_t out_dtype;                 /* of y and residual: dtype or SSMAP_F32 */
@@ -383,7 +383,7 @@ int ssmap_linear(const ssmap_linear_args *args, void *stream);
 
 /* The gradients of ssmap_linear from g = dL/dy.  With dz = g act'(pre):
  *   g_x = dz w,   g_w = dz^T x,   g_bias = sum of dz over the positions   (g itself is the residual's).
- * Where dtype has 16 bits and g is float32 or an activation is given, dz goes into the two products as two values of
+ * Where dtype has 16 bits and g is float32 or an activation other than relu is given, dz goes into the two products as two values of
  * dtype, the rounded one and what the rounding left (the matrix instructions' operands have no more bits): 16 bits of
  * it for SSMAP_BF16, 22 for SSMAP_F16, there scaled by the power of two that the largest finite |g| asks for (what lies
  * below 2^-38 of that is lost).  An infinite x or w then can make NaN of what the formulas call infinite.

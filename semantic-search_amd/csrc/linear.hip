@@ -308,7 +308,8 @@ GradPlan plan_grad(const ssmap_linear_grad_args *a) {
     const int64_t chunk = q.planes ? kDzPlane : kDzRows;
     q.chunks = a->batch * ((a->rows + chunk - 1) / chunk);
     const int64_t values = a->batch * (q.planes ? a->outer : a->rows) * q.dz_line;
-    q.dz_rest = a->dtype != SSMAP_F32 && (a->activation != SSMAP_ACT_NONE || a->grad_dtype != a->dtype) ? values : 0;
+    const bool slopes = a->activation != SSMAP_ACT_NONE && a->activation != SSMAP_ACT_RELU;   // relu's are 0 and 1: exact
+    q.dz_rest = a->dtype != SSMAP_F32 && (slopes || a->grad_dtype != a->dtype) ? values : 0;
     const int64_t parts = q.dz_rest ? 2 : 1;
     q.dz_bytes = q.copies && (a->g_x || a->g_w) ? aligned(parts * values * size) : 0;
     q.scale_bytes = q.dz_bytes && q.dz_rest && a->dtype == SSMAP_F16 ? aligned((2 + kPeaks) * 4) : 0;

@@ -185,3 +185,16 @@ def test_tangents_are_seen():
         assert heads._tangent(dual) and not heads._tangent(t)
         with torch.no_grad():
             assert heads._tangent(dual) and not heads._tangent(forward_ad.unpack_dual(dual).primal)
+
+
+def test_dz_is_kept_twice_where_16_bits_do_not_hold_it():
+    """Parts of dz in the workspace: a float32 gradient and slopes between 0 and 1 round, relu's and none do not."""
+    sizes = dict(layout=0, rows=512, inner=64, outer=64, g_inner_stride=64, x_row_stride=64, w_row_stride=64, pre=16)
+    one = 512 * 64 * 2
+    dz = lambda dtype, g, act: _grad_workspace(**sizes, dtype=dtype, grad_dtype=g, activation=act, g_x=16) - \
+        _grad_workspace(**sizes, dtype=dtype, grad_dtype=dtype, activation=0, g_x=16)  # noqa: E731
+    for dtype, scale in ((1, 0), (2, 4352)):      # fp16: its scale and the blocks' peaks as well
+        assert dz(dtype, dtype, 1) == one
+        assert [dz(dtype, dtype, act) for act in (2, 3, 4)] == [2 * one + scale] * 3
+        assert [dz(dtype, 0, act) for act in (0, 1, 2)] == [2 * one + scale] * 3
+    assert dz(0, 0, 2) == 2 * one                 # float32: once
