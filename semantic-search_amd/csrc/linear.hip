@@ -325,7 +325,7 @@ GradPlan plan_grad(const ssmap_linear_grad_args *a) {
     x.a = dz; x.a_out = batch; x.a_sum = q.dz_rest; x.a_m = to_row; x.a_k = to_out;
     x.b = a->w; x.b_n = 1; x.b_k = a->w_row_stride;
     x.out = a->g_x;
-    w.M = a->outer; w.N = a->inner; w.K = a->rows; w.out_batches = 1; w.sum_batches = parts * a->batch; w.b_again = a->batch;
+    w.M = a->outer; w.N = a->inner; w.K = a->rows; w.out_batches = 1; w.sum_batches = parts * a->batch; w.b_again = a->batch ? a->batch : 1;
     w.a = dz; w.a_sum = batch; w.a_m = to_out; w.a_k = to_row;
     w.b = a->x; w.b_sum = a->x_batch_stride; w.b_n = 1; w.b_k = a->x_row_stride;
     w.out = a->g_w;

@@ -914,6 +914,18 @@ def test_slope_where_pre_is_infinite(dtype, act):
         assert torch.isnan(ssa.linear_grad(g, x, w, activation=act, pre=pre).x[2, 0])
 
 
+def test_linear_grad_of_no_frames():
+    for dtype in TYPES:
+        w = torch.ones((4, 8), dtype=dtype, device="cuda")
+        for act in (None, "silu"):
+            dy = torch.zeros((0, 4, 9), dtype=torch.float32 if act is None else dtype, device="cuda")
+            g = ssa.linear_grad(dy, torch.zeros((0, 9, 8), dtype=dtype, device="cuda"), w, activation=act, pre=dy.to(dtype) if act else None, planes=True)
+            assert g.x.shape == (0, 9, 8) and not g.weight.any() and not g.bias.any() and g.weight.shape == (4, 8)
+            dy = dy.new_zeros((0, 9, 4))
+            g = ssa.linear_grad(dy, torch.zeros((0, 9, 8), dtype=dtype, device="cuda"), w, activation=act, pre=dy.to(dtype) if act else None)
+            assert g.x.shape == (0, 9, 8) and not g.weight.any() and not g.bias.any()
+
+
 # ------------------------------------------------------------------ together, streams, graphs, the engine
 
 def test_a_training_step_of_a_head():
@@ -1040,6 +1052,60 @@ def test_two_streams_at_once():
         for k in range(2):
             with torch.cuda.stream(streams[k]):
                 got[k].append(_step(*ins[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for run in got[k]:
+            for a, want in zip(run, wants[k]):
+                assert torch.equal(a, want)
+
+
+def _head_step(x, w, b, ids):
+    y, pre = ssa.linear(x, w, b, activation="gelu", planes=True, out_dtype=torch.float32, keep_pre=True)
+    s = ssa.log_probs(y, ids, dim=1, top=2)
+    gl = ssa.log_probs_grad(y, ids, s, dim=1, grad_log_prob=torch.full_like(s.log_prob, -1e-7), grad_top=torch.full_like(s.top_log_prob, 1e-8))
+    return (y,) + tuple(s) + (gl,) + tuple(ssa.linear_grad(gl, x, w, activation="gelu", pre=pre, planes=True))
+
+
+def _head_inputs(seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn((2, 600, 96), device="cuda", generator=g).half()
+    w = torch.randn((21, 96), device="cuda", generator=g).half() * 0.2
+    return x, w, torch.randn((21,), device="cuda", generator=g), torch.randint(0, 21, (2, 600), device="cuda", generator=g)
+
+
+def test_a_float16_head_in_two_graphs_and_streams():
+    """The gradient's scale comes from each call's own values: two graphs replayed in turn with eager work between
+    them, and two streams at once, against eager results."""
+    stills, graphs, outs = [_head_inputs(1), _head_inputs(2)], [], []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _head_step(*stills[0])
+    torch.cuda.current_stream().wait_stream(side)
+    for s in stills:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(_head_step(*s))
+        graphs.append(graph)
+    for turn in range(4):
+        fresh = [_head_inputs(10 + 2 * turn + k) for k in range(2)]
+        fresh[1][1].mul_(3.0 ** turn)
+        wants = [[t.clone() for t in _head_step(*f)] for f in fresh]
+        for k in range(2):
+            for a, f in zip(stills[k], fresh[k]):
+                a.copy_(f)
+        for k in (0, 1, 0):
+            graphs[k].replay()
+        torch.cuda.synchronize()
+        for k in range(2):
+            for a, want in zip(outs[k], wants[k]):
+                assert torch.equal(a, want), (turn, k)
+        assert wants[0][-2].any()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(5):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(_head_step(*fresh[k]))
     torch.cuda.synchronize()
     for k in range(2):
         for run in got[k]:
