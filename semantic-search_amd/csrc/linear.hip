@@ -22,7 +22,7 @@ inline bool direct_side(const void *p, int64_t line, int64_t out, int64_t sum, i
 
 // dz = g act'(pre) in the products' type, dense, and the sums of its positions for the bias's gradient, in one
 // pass over g.  [batch][P][Q], Q dense: rows have the outputs in Q, planes in P.  8192 x 4096 bf16 with gelu takes
-// 47 us (the bytes 39): the slope's two transcendentals a value fill the rest.
+// 85 us (the bytes 52): the slope's two transcendentals a value and both parts' roundings fill the rest.
 //
 // Where 16 bits do not hold dz it is kept as two values, the rounded one and what the rounding left, and the products
 // sum over both: dz then counts with 2^-16 (bf16) or 2^-22 (fp16) of its size, and a result is rounded once, as the
@@ -33,6 +33,7 @@ inline bool direct_side(const void *p, int64_t line, int64_t out, int64_t sum, i
 // fp16 holds nothing above 65504 and little below 2^-14, where a float32 gradient averaged over a frame's positions
 // lies.  There dz is multiplied by the power of two that brings the largest finite |g| to 2^13 ... 2^14 (no slope exceeds
 // 1.13), and the products' sums by its inverse: what is lost of a value is at most 2^-38 of that largest one.
+// The look at g takes 11 us for 40 planes of 307200 positions (4.6 TB/s), the scale 4.
 constexpr int kDzRows = 128;       // rows: positions a block sums; 8 threads down, 32 packs of 8 outputs across
 constexpr int kDzPlane = 16384;    // planes: positions a block sums
 

@@ -539,7 +539,7 @@ constexpr int kPlaneClasses = 8;   // classes a plane kernel holds in flight
 // what the additions round off kept aside (true value: sum - sum_off); and the sums are rescaled only where a logit
 // exceeds their reference by more than a factor of two in its exponential, so that what a rescaling rounds fades by
 // half with the next.  K >= s.top.  Bound by memory: 16 x 40 x 480 x 640 float32 with three alternatives takes
-// 207 us, 4.8 TB/s (fetching the given class afterwards and storing position by position 368 us).
+// 205 us, 4.8 TB/s (fetching the given class afterwards and storing position by position 368 us).
 // With five alternatives the registers stand at the border of five waves a SIMD (96): asked for, 250 and 301 us in
 // float32 and 16 bits; left to the compiler, which takes 97, 256 and 344.
 template <int DT, int PX, int K>
