@@ -926,6 +926,41 @@ def test_linear_grad_of_no_frames():
             assert g.x.shape == (0, 9, 8) and not g.weight.any() and not g.bias.any()
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("n", [(1 << 21) + 3, (1 << 21) + 8])
+def test_linear_grad_of_planes_past_the_direct_loads(n, dtype):
+    """Planes of more than 2^21 positions, whose lines are too far apart for 32-bit offsets within a tile: loads
+    through registers, dz in parts, two frames in the weight's sum."""
+    E, K, N = 2, 8, 5
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn((E, n, K), device="cuda", generator=g).to(dtype)
+    w = (torch.randn((N, K), device="cuda", generator=g) / 4).to(dtype)
+    dy = torch.randn((E, N, n), device="cuda", generator=g).to(dtype)
+    pre = (torch.randn(dy.shape, device="cuda", generator=g) * 1.5).to(dtype)
+    for act in (None, "silu"):
+        got = ssa.linear_grad(dy, x, w, activation=act, pre=pre if act else None, planes=True)
+        want, size, gsize = plain_linear_grad(dy, x, w, act, pre if act else None, True)
+        check_grad_rounded_once(got, want, size, gsize, E * n, N, w, x, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids_of)
+@pytest.mark.parametrize("planes", [False, True])
+def test_linear_grad_of_expanded_operands(planes, dtype):
+    """One frame's features, gradients and weights standing for several: strides of 0 along batch, rows and outputs."""
+    B, n, K, N = 3, 300, 72, 70
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.randn((1, n, K), device="cuda", generator=g).to(dtype).expand(B, n, K)
+    w = (torch.randn((1, K), device="cuda", generator=g) / 8).to(dtype).expand(N, K)
+    dy = torch.randn((1, N, n) if planes else (1, n, N), device="cuda", generator=g).to(dtype)
+    dy = dy.expand((B,) + dy.shape[1:])
+    pre = (torch.randn(dy.shape, device="cuda", generator=g) * 1.5).to(dtype)
+    assert torch.equal(ssa.linear(x, w, planes=planes), ssa.linear(x.contiguous(), w.contiguous(), planes=planes))
+    for act in (None, "gelu"):
+        got = ssa.linear_grad(dy, x, w, activation=act, pre=pre if act else None, planes=planes)
+        want, size, gsize = plain_linear_grad(dy, x, w, act, pre if act else None, planes)
+        check_grad_rounded_once(got, want, size, gsize, B * n, N, w, x, dtype)
+
+
 # ------------------------------------------------------------------ together, streams, graphs, the engine
 
 def test_a_training_step_of_a_head():
